@@ -35,9 +35,10 @@
 extern "C" {
 #endif
 
-#define MI_PAGED_ABI_VERSION 4  /* 2: mi_paged_decode_workspace_bytes takes num_kv_heads;
+#define MI_PAGED_ABI_VERSION 5  /* 2: mi_paged_decode_workspace_bytes takes num_kv_heads;
                                    3: mi_paged_decode_attention_exact takes a workspace;
-                                   4: mi_mixed_paged_attention[_exact] take ragged chunk rows */
+                                   4: mi_mixed_paged_attention[_exact] take ragged chunk rows;
+                                   5: the 4-bit pools (mi_*_fp4) and mi_copy_blocks */
 
 #define MI_OK 0
 #define MI_ERR_INVALID_ARGUMENT (-1) /* null pointer, negative size, bad stride  */
@@ -473,6 +474,89 @@ int32_t mi_pack_blocks(void* records, const void* const* key_pools, const void* 
 int32_t mi_unpack_blocks(void* const* key_pools, void* const* value_pools, int64_t num_blocks,
                          const void* records, const int64_t* block_ids, int64_t num_records, int32_t num_layers,
                          int64_t block_bytes, void* stream);
+
+/*
+ * Block copies inside the pools: block dst_blocks[i] = block src_blocks[i] of every layer, K and V.  For forks (a
+ * continuation's own copy of the block its parent goes on writing) and compaction (live blocks moved to free ones);
+ * the reference only hands blocks out and frees them (src/mini_infra/core/block_manager.py:35-76).
+ * key_pools / value_pools: num_layers device pointers, each num_blocks * block_bytes, of any type and layout.
+ * src_blocks / dst_blocks: device int64 [num_pairs].  Destinations must be unique, and none may be the source of
+ * another pair of the call (the copies run side by side); a block may be the source of many.  A source outside
+ * [0, num_blocks) reads the null block 0, a pair with a destination outside it, or with equal ids, is skipped.
+ */
+int32_t mi_copy_blocks(void* const* key_pools, void* const* value_pools, int64_t num_blocks,
+                       const int64_t* src_blocks, const int64_t* dst_blocks, int64_t num_pairs, int32_t num_layers,
+                       int64_t block_bytes, void* stream);
+
+/*
+ * The 4-bit cache (MXFP4): K/V pools of 4.25 bits a value instead of 16, and the entry points of kernels 1 to 4 over them.
+ *
+ * A row of 128 values (one token of one KV head) is four groups of 32 dims.  A group has a scale byte c (E8M0: 2^(c - 127);
+ * 255 is NaN) and 32 codes of 4 bits (E2M1: bit 3 the sign, magnitudes 0, 0.5, 1, 1.5, 2, 3, 4, 6); a value is
+ * code x scale.  With a the group's largest magnitude, c = clamp(((bits(fp32 a) + 2^21) >> 23) - 2, 1, 252), the
+ * smallest scale at which a rounds to at most 6; codes are rounded to nearest, ties to the even code, saturated at
+ * 6.  A group with an infinity or NaN gets c = 255 and reads as NaN.
+ *
+ * A pool is bytes [num_blocks, num_kv_heads, 1088] in blocks of 16 tokens (a pool of block_size 16 k is the same memory as
+ * one of k times as many blocks of 16), 16-byte aligned.  The record of one block and KV head, two codes a byte, the
+ * even dim in the low four bits:
+ *   K: codes [4 groups][16 tokens][16 bytes],              scales [4 groups][16 tokens]
+ *   V: codes [4 token quads][16 dim octets][4 tokens][4 bytes], scales [4 token quads][4 groups][4 tokens]
+ * A zero-filled pool reads as zeros.  Whole blocks are copied, packed and swapped as bytes (mi_copy_blocks,
+ * mi_pack_blocks, block_bytes = num_kv_heads * 1088).  num_kv_heads may be any positive number; head_dim is 128.
+ *
+ * mi_reshape_and_cache_fp4 -- mi_reshape_and_cache with quantisation: the same sources, index arrays and skipping rules; source
+ * elements of type src_type, any strides with head_dim contiguous; num_slots = 16 x blocks.
+ *
+ * mi_gather_blocks_fp4 -- mi_gather_blocks as values: key_out[l][b, 16 j + t, h, :] = the bf16 values (exact) of block
+ * block_ids[b * block_id_stride + j], outputs contiguous [batch, 16 * num_gathered_blocks, num_kv_heads, 128].
+ *
+ * mi_paged_decode_attention_fp4 -- kernel 3 over 4-bit pools: the arguments of mi_paged_decode_attention (without block_size), the
+ * same visibility, zero rows for contexts <= 0, and
+ *   out[b, h] = bf16( sum_{t < n} softmax(scale q . K_t) V_t )
+ * with scores, softmax and sums in fp32 (weights rounded to bf16 for the product with V).  At most 8 query heads per KV
+ * head.  Tokens past a context never reach its output, whatever their bytes hold.  workspace: at least
+ * mi_paged_decode_fp4_workspace_bytes(...) bytes, which depends on the device's CU count, of this call's own while it runs (NULL
+ * where that is 0); no initialisation needed.
+ *
+ * mi_chunked_prefill_attention_fp4 -- kernel 4 with the history in 4-bit pools and the chunk's own K/V in bf16: the arguments of
+ * mi_chunked_prefill_attention (without block_size) and its visibility, scores in fp32.  Padding positions of the
+ * chunk and history slots past start_lens never reach an output; the chunk's real K and V rows are taken to be finite
+ * (one that is not may also reach queries before it).  max_history_blocks is not limited by LDS.
+ */
+#define MI_TYPE_BF16 1
+#define MI_TYPE_FP16 2
+#define MI_TYPE_FP32 3
+int32_t mi_reshape_and_cache_fp4(const void* const* key_src, const void* const* value_src, int64_t key_row_stride,
+                                 int64_t key_head_stride, int64_t key_pos_stride, int64_t value_row_stride,
+                                 int64_t value_head_stride, int64_t value_pos_stride, const int64_t* token_rows,
+                                 const int64_t* token_positions, const int64_t* slot_mapping, int64_t index_stride,
+                                 int64_t num_tokens, int64_t num_src_rows, int64_t num_src_positions,
+                                 void* const* key_pools, void* const* value_pools, int32_t num_layers,
+                                 int64_t num_slots, int32_t num_kv_heads, int32_t head_dim, int32_t src_type,
+                                 void* stream);
+int32_t mi_gather_blocks_fp4(const void* const* key_pools, const void* const* value_pools, int64_t num_blocks,
+                             const int64_t* block_ids, int64_t block_id_stride, int32_t batch,
+                             int32_t num_gathered_blocks, void* const* key_out, void* const* value_out,
+                             int32_t num_layers, int32_t num_kv_heads, int32_t head_dim, void* stream);
+int64_t mi_paged_decode_fp4_workspace_bytes(int32_t batch, int32_t max_blocks, int32_t num_heads,
+                                            int32_t num_kv_heads);
+int32_t mi_paged_decode_attention_fp4(void* out, int64_t out_row_stride, const void* query, int64_t query_row_stride,
+                                      int64_t query_head_stride, const void* key_pool, const void* value_pool,
+                                      int64_t num_blocks, const int64_t* block_tables, int64_t block_table_stride,
+                                      int32_t max_blocks, const int64_t* context_lens, int64_t context_lens_stride,
+                                      int32_t batch, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                                      float scale, void* workspace, int64_t workspace_bytes, void* stream);
+int32_t mi_chunked_prefill_attention_fp4(void* out, int64_t out_row_stride, int64_t out_tok_stride, const void* query,
+                                         int64_t query_row_stride, int64_t query_head_stride, int64_t query_tok_stride,
+                                         const void* key, int64_t key_row_stride, int64_t key_head_stride,
+                                         int64_t key_tok_stride, const void* value, int64_t value_row_stride,
+                                         int64_t value_head_stride, int64_t value_tok_stride, const void* key_pool,
+                                         const void* value_pool, int64_t num_blocks, const int64_t* history_blocks,
+                                         int64_t history_stride, int32_t max_history_blocks, const int64_t* start_lens,
+                                         const int64_t* chunk_lens, int64_t lens_stride, int32_t batch,
+                                         int32_t padded_len, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                                         float scale, void* stream);
 
 #ifdef __cplusplus
 }

@@ -15,13 +15,17 @@ from pathlib import Path
 import torch  # noqa: F401  (must be imported before the library; see module docstring)
 
 LIBRARY_PATH = Path(__file__).resolve().with_name("libmi_paged.so")
-ABI_VERSION = 4
+ABI_VERSION = 5
 
 MI_OK = 0
 MI_ERR_INVALID_ARGUMENT = -1
 MI_ERR_UNSUPPORTED = -2
 MI_ERR_WORKSPACE = -3
 MI_ERR_DEVICE = -4
+
+MI_TYPE_BF16 = 1
+MI_TYPE_FP16 = 2
+MI_TYPE_FP32 = 3
 
 _c_void_p_p = ctypes.POINTER(ctypes.c_void_p)
 _i32 = ctypes.c_int32
@@ -107,6 +111,27 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "mi_argmax_rows": (_i32, [_ptr, _ptr, _i64, _i32, _i64, _ptr]),
     "mi_pack_blocks": (_i32, [_ptr, _c_void_p_p, _c_void_p_p, _i64, _ptr, _i64, _i32, _i64, _ptr]),
     "mi_unpack_blocks": (_i32, [_c_void_p_p, _c_void_p_p, _i64, _ptr, _ptr, _i64, _i32, _i64, _ptr]),
+    "mi_copy_blocks": (_i32, [_c_void_p_p, _c_void_p_p, _i64, _ptr, _ptr, _i64, _i32, _i64, _ptr]),
+    "mi_reshape_and_cache_fp4": (
+        _i32,
+        [_c_void_p_p, _c_void_p_p, _i64, _i64, _i64, _i64, _i64, _i64, _ptr, _ptr, _ptr, _i64, _i64, _i64, _i64,
+         _c_void_p_p, _c_void_p_p, _i32, _i64, _i32, _i32, _i32, _ptr],
+    ),
+    "mi_gather_blocks_fp4": (
+        _i32,
+        [_c_void_p_p, _c_void_p_p, _i64, _ptr, _i64, _i32, _i32, _c_void_p_p, _c_void_p_p, _i32, _i32, _i32, _ptr],
+    ),
+    "mi_paged_decode_fp4_workspace_bytes": (_i64, [_i32, _i32, _i32, _i32]),
+    "mi_paged_decode_attention_fp4": (
+        _i32,
+        [_ptr, _i64, _ptr, _i64, _i64, _ptr, _ptr, _i64, _ptr, _i64, _i32, _ptr, _i64, _i32, _i32, _i32, _i32,
+         ctypes.c_float, _ptr, _i64, _ptr],
+    ),
+    "mi_chunked_prefill_attention_fp4": (
+        _i32,
+        [_ptr, _i64, _i64, _ptr, _i64, _i64, _i64, _ptr, _i64, _i64, _i64, _ptr, _i64, _i64, _i64, _ptr, _ptr, _i64,
+         _ptr, _i64, _i32, _ptr, _ptr, _i64, _i32, _i32, _i32, _i32, _i32, ctypes.c_float, _ptr],
+    ),
 }
 
 

@@ -128,17 +128,6 @@ __device__ __forceinline__ void reference_scores(f32x4& v, float scale) {
   for (int i = 0; i < 4; ++i) v[i] = round_bf16(round_bf16(v[i]) * scale);
 }
 
-// One 16-byte-per-lane load straight into LDS, from a uniform base and a byte offset per lane: lane i
-// writes bytes [16 i, 16 i + 16) of the 1 KiB span at LDS address lds (wave-uniform, passed in M0; one wait state between the M0 write
-// and the load).  Issued by inline assembly: the compiler's own form ties every later LDS read to
-// the completion of all such loads (it cannot tell the two tile buffers apart), which would wait
-// for tile t + 1 before reading tile t.  The compiler does not see these loads, so the kernel waits
-// for them itself (vmcnt(0) before each tile barrier).  The LDS address goes in through an M0
-// operand constraint, so the compiler writes M0 itself and knows its value across the asm.
-__device__ __forceinline__ void dma16(const void* base, uint32_t off, uint32_t lds) {
-  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "{m0}"(lds) : "memory");
-}
-
 // A decode row of a mixed step (its single new token) by one workgroup of kStripes wavefronts per KV head,
 // with the arithmetic of the decode kernels: stripe v attends blocks v, v + kStripes, ... of the history
 // and the token, whose K and V rows (not yet in the pool, and appended here) are put in place of what its

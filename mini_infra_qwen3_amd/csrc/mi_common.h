@@ -61,6 +61,21 @@ __device__ __forceinline__ void store_stream(T* p, const T& v) {
   }
 }
 
+// One 16-byte-per-lane load straight into LDS, from a uniform base and a byte offset per lane: lane i
+// writes bytes [16 i, 16 i + 16) of the 1 KiB span at LDS address lds (wave-uniform, passed in M0; one wait state between the M0 write
+// and the load).  Issued by inline assembly: the compiler's own form ties every later LDS read to
+// the completion of all such loads (it cannot tell the two tile buffers apart), which would wait
+// for tile t + 1 before reading tile t.  The compiler does not see these loads, so the kernel waits
+// for them itself (vmcnt(0) before each tile barrier).  The LDS address goes in through an M0
+// operand constraint, so the compiler writes M0 itself and knows its value across the asm.
+// A base that a vector instruction wrote (v_readfirstlane of a pointer) needs five wait states before the load reads
+// it, which the compiler keeps for its own loads but not for the asm: such callers pass kWaits = 5.  The
+// default is for bases that come out of scalar arithmetic.
+template <int kWaits = 1>
+__device__ __forceinline__ void dma16(const void* base, uint32_t off, uint32_t lds) {
+  asm volatile("s_nop %3\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "{m0}"(lds), "n"(kWaits - 1) : "memory");
+}
+
 inline hipStream_t as_stream(void* s) { return reinterpret_cast<hipStream_t>(s); }
 
 // An out-of-range block id reads the null block 0, which an empty pool does not have: a call that

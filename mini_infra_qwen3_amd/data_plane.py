@@ -15,18 +15,26 @@ import torch
 from mini_infra_qwen3_amd import _native
 
 __all__ = [
+    "FP4_RECORD_BYTES",
     "KERNEL_BLOCK_SIZE",
     "argmax_rows",
     "chunked_prefill_attention",
+    "chunked_prefill_attention_fp4",
+    "copy_blocks",
+    "fp4_pool_shape",
     "gather_blocks",
+    "gather_blocks_fp4",
     "mixed_paged_attention",
     "pack_blocks",
     "paged_decode_attention",
+    "paged_decode_attention_fp4",
     "paged_decode_attention_fused",
     "paged_decode_exact_workspace_bytes",
+    "paged_decode_fp4_workspace_bytes",
     "paged_decode_workspace_bytes",
     "qk_norm_rope",
     "reshape_and_cache",
+    "reshape_and_cache_fp4",
     "rms_norm",
     "set_index_checks",
     "silu_mul",
@@ -249,8 +257,13 @@ def _as_kernel_blocks(key_pool: torch.Tensor, value_pool: torch.Tensor, tables: 
     n = key_pool.shape[0]
     kp = key_pool.view(n * k, KERNEL_BLOCK_SIZE, *key_pool.shape[2:])
     vp = value_pool.view(n * k, KERNEL_BLOCK_SIZE, *value_pool.shape[2:])
+    return kp, vp, _sub_block_ids(tables, k)
+
+
+def _sub_block_ids(tables: torch.Tensor, k: int) -> torch.Tensor:
+    """``[B, nb * k]`` ids of the k sub-blocks of every entry of ``tables [B, nb]``."""
     sub = torch.arange(k, dtype=tables.dtype, device=tables.device)
-    return kp, vp, (tables.unsqueeze(-1) * k + sub).reshape(tables.shape[0], tables.shape[1] * k)
+    return (tables.unsqueeze(-1) * k + sub).reshape(tables.shape[0], tables.shape[1] * k)
 
 
 def paged_decode_workspace_bytes(batch: int, max_blocks: int, num_heads: int, head_dim: int, block_size: int,
@@ -897,3 +910,338 @@ def unpack_blocks(records: torch.Tensor, key_pools: Sequence[torch.Tensor], valu
         _native.pointer_array([t.data_ptr() for t in value_pools]), pool0.shape[0], records.data_ptr(),
         block_ids.data_ptr(), block_ids.shape[0], len(key_pools), block_bytes, _stream(device))
     _native.check(rc, "mi_unpack_blocks")
+
+
+def copy_blocks(key_pools: Sequence[torch.Tensor], value_pools: Sequence[torch.Tensor], src_blocks: torch.Tensor,
+                dst_blocks: torch.Tensor) -> None:
+    """Copies whole physical blocks of every layer to other blocks of the same pools (one launch): block
+    ``dst_blocks[i]`` becomes block ``src_blocks[i]``, K and V.
+
+    Pools ``[num_blocks, ...]`` of any dtype, 4-bit ones included.  src_blocks / dst_blocks: ``[n]`` int64 on the
+    pools' device.  Destinations are unique and none is the source of another pair (the copies run side by
+    side); a block may be the source of many.  A source outside ``[0, num_blocks)`` reads the null block 0,
+    a pair with a destination outside it is skipped; with ``set_index_checks`` on either raises
+    ``IndexError``, and destinations that break the rule above raise ``ValueError``.
+    """
+    pool0, device, block_bytes = _record_pools(key_pools, value_pools)
+    for name, t in (("src_blocks", src_blocks), ("dst_blocks", dst_blocks)):
+        _require_gpu(name, t, device)
+        _require_index(name, t, 1)
+    if src_blocks.shape != dst_blocks.shape:
+        raise ValueError(f"{src_blocks.shape[0]} source blocks for {dst_blocks.shape[0]} destinations")
+    if src_blocks.shape[0] == 0:
+        return
+    _check_range("src_blocks", src_blocks, pool0.shape[0])
+    _check_range("dst_blocks", dst_blocks, pool0.shape[0])
+    if _INDEX_CHECKS:
+        if torch.unique(dst_blocks).numel() != dst_blocks.numel():
+            raise ValueError("dst_blocks: a block is written twice")
+        moved = dst_blocks[dst_blocks != src_blocks]
+        if bool(torch.isin(moved, src_blocks).any()):
+            raise ValueError("dst_blocks: a block that is written is also a source")
+    src_blocks, dst_blocks = src_blocks.contiguous(), dst_blocks.contiguous()
+    _call(device, "mi_copy_blocks", _native.pointer_array([t.data_ptr() for t in key_pools]),
+          _native.pointer_array([t.data_ptr() for t in value_pools]), pool0.shape[0], src_blocks.data_ptr(),
+          dst_blocks.data_ptr(), src_blocks.shape[0], len(key_pools), block_bytes, _stream(device))
+
+
+# ------------------------------------------------------------------------------ the 4-bit cache
+FP4_RECORD_BYTES = 1088  # 16 tokens of one KV head: 1024 bytes of 4-bit codes, 64 scale bytes
+_FP4_SOURCE_TYPES = {torch.bfloat16: _native.MI_TYPE_BF16, torch.float16: _native.MI_TYPE_FP16,
+                     torch.float32: _native.MI_TYPE_FP32}
+
+
+def fp4_pool_shape(num_blocks: int, block_size: int, num_kv_heads: int, head_dim: int = 128) -> tuple[int, int, int, int]:
+    """Shape ``[num_blocks, block_size / 16, num_kv_heads, 1088]`` of one layer's 4-bit key or value pool (uint8).
+
+    MXFP4: a row of 128 values is four groups of 32 with a power-of-two scale byte each and 4-bit codes
+    (magnitudes 0, 0.5, 1, 1.5, 2, 3, 4, 6 times the scale).  The bytes of a record are laid out for the
+    kernels (``include/mi_paged.h``); blocks are copied, packed and swapped whole, as bytes.
+    """
+    if head_dim != 128:
+        raise ValueError(f"4-bit pools need head_dim 128, got {head_dim}")
+    if block_size < KERNEL_BLOCK_SIZE or block_size % KERNEL_BLOCK_SIZE != 0:
+        raise ValueError(f"4-bit pools need a block_size that is a multiple of {KERNEL_BLOCK_SIZE}, got {block_size}")
+    if num_blocks < 0 or num_kv_heads < 1:
+        raise ValueError("4-bit pools need num_blocks >= 0 and num_kv_heads >= 1")
+    return num_blocks, block_size // KERNEL_BLOCK_SIZE, num_kv_heads, FP4_RECORD_BYTES
+
+
+def _call(device: torch.device, name: str, *args) -> None:
+    """Calls an entry point with the tensors' device current (a launch goes to the current device's runtime state)."""
+    entry = getattr(_native.load(), name)
+    if torch._C._cuda_getDevice() == device.index:
+        rc = entry(*args)
+    else:
+        with torch.cuda.device(device):
+            rc = entry(*args)
+    _native.check(rc, name)
+
+
+def _require_fp4_pools(key_pools: Sequence[torch.Tensor], value_pools: Sequence[torch.Tensor]) -> torch.Tensor:
+    """Checks 4-bit pools (one shape, one device, contiguous uint8); returns the first."""
+    pool0 = key_pools[0]
+    shape, device = pool0.shape, pool0.device
+    if pool0.ndim != 4 or shape[1] < 1 or shape[2] < 1 or shape[3] != FP4_RECORD_BYTES:
+        raise ValueError(f"4-bit pools must be [num_blocks, block_size / 16, H_kv, {FP4_RECORD_BYTES}], got {tuple(shape)}")
+    index = pool0.get_device()
+    for name, tensors in (("key_pools", key_pools), ("value_pools", value_pools)):
+        for t in tensors:
+            if index < 0 or t.get_device() != index:
+                _require_gpu(name, t, device)
+            if t.shape != shape or t.dtype is not torch.uint8 or not t.is_contiguous():
+                raise ValueError(f"{name}: every 4-bit pool must be contiguous {tuple(shape)} uint8, got "
+                                 f"{tuple(t.shape)} {t.dtype}")
+    return pool0
+
+
+def _fp4_sub_block_ids(tables: torch.Tensor, num_blocks: int, sub: int) -> torch.Tensor:
+    """``_sub_block_ids`` with ids outside ``[0, num_blocks)`` as the null block's sub-blocks."""
+    return _sub_block_ids(torch.where((tables >= 0) & (tables < num_blocks), tables, 0), sub)
+
+
+def reshape_and_cache_fp4(
+    key_src: Sequence[torch.Tensor],
+    value_src: Sequence[torch.Tensor],
+    slot_mapping: torch.Tensor,
+    key_pools: Sequence[torch.Tensor],
+    value_pools: Sequence[torch.Tensor],
+    token_rows: torch.Tensor | None = None,
+    token_positions: torch.Tensor | None = None,
+) -> None:
+    """``reshape_and_cache`` into 4-bit pools (``fp4_pool_shape``): K/V rows of every layer, quantised into their
+    slots in one launch.
+
+    key_src[l] / value_src[l]: ``[B, H_kv, L, 128]`` bf16, fp16 or fp32 (any strides with D contiguous, the same in
+    every layer); slot_mapping / token_rows / token_positions: ``[N]`` int64, as there; slots must be unique.
+    A group of 32 dims that holds an infinity or NaN is stored as NaN.
+    """
+    num_layers = len(key_pools)
+    if not (len(key_src) == len(value_src) == len(value_pools) == num_layers):
+        raise ValueError("reshape_and_cache_fp4: per-layer lists differ in length")
+    if num_layers == 0:
+        return
+    pool0 = _require_fp4_pools(key_pools, value_pools)
+    device, index = pool0.device, pool0.get_device()
+    num_blocks, sub, num_kv_heads, _ = pool0.shape
+    k0, v0 = key_src[0], value_src[0]
+    dtype = k0.dtype
+    if dtype not in _FP4_SOURCE_TYPES:
+        raise ValueError(f"key_src must be bf16, fp16 or fp32, got {dtype}")
+    for name, tensors, ref in (("key_src", key_src, k0), ("value_src", value_src, v0)):
+        shape, stride = ref.shape, ref.stride()
+        if len(shape) != 4 or shape[1] != num_kv_heads or shape[3] != 128:
+            raise ValueError(f"{name} must be [B, {num_kv_heads}, L, 128], got {tuple(shape)}")
+        for t in tensors:
+            if t.get_device() != index:
+                _require_gpu(name, t, device)
+            if t.dtype is not dtype or t.shape != shape or t.stride() != stride or stride[3] != 1:
+                raise ValueError(f"{name}: all layers need {dtype} and the same shape and strides, with D contiguous")
+    if k0.shape != v0.shape:
+        raise ValueError("reshape_and_cache_fp4: key and value sources differ in shape")
+    num_tokens = slot_mapping.shape[0] if slot_mapping.ndim else 0
+    indices = [slot_mapping, token_rows, token_positions]
+    for name, t in zip(("slot_mapping", "token_rows", "token_positions"), indices):
+        if t is not None:
+            _require_gpu(name, t, device)
+            _require_index(name, t, 1)
+            if t.shape[0] != num_tokens:
+                raise ValueError(f"{name} has {t.shape[0]} entries, slot_mapping {num_tokens}")
+    if num_tokens == 0:
+        return
+    _check_range("slot_mapping", slot_mapping, num_blocks * sub * KERNEL_BLOCK_SIZE, allow_minus_one=True)
+    if token_rows is not None:
+        _check_range("token_rows", token_rows, k0.shape[0])
+    if token_positions is not None:
+        _check_range("token_positions", token_positions, k0.shape[2])
+    index_stride = slot_mapping.stride(0) if num_tokens > 1 else 1
+    if num_tokens > 1 and (index_stride <= 0 or any(t is not None and t.stride(0) != index_stride for t in indices)):
+        indices = [None if t is None else t.contiguous() for t in indices]
+        index_stride = 1
+    slots, rows, positions = indices
+    _call(device, "mi_reshape_and_cache_fp4",
+          _native.pointer_array([t.data_ptr() for t in key_src]), _native.pointer_array([t.data_ptr() for t in value_src]),
+          k0.stride(0), k0.stride(1), k0.stride(2), v0.stride(0), v0.stride(1), v0.stride(2),
+          rows.data_ptr() if rows is not None else None, positions.data_ptr() if positions is not None else None,
+          slots.data_ptr(), index_stride, num_tokens, k0.shape[0], k0.shape[2],
+          _native.pointer_array([t.data_ptr() for t in key_pools]),
+          _native.pointer_array([t.data_ptr() for t in value_pools]), num_layers,
+          num_blocks * sub * KERNEL_BLOCK_SIZE, num_kv_heads, 128, _FP4_SOURCE_TYPES[dtype], _stream(device))
+
+
+def gather_blocks_fp4(
+    key_pools: Sequence[torch.Tensor],
+    value_pools: Sequence[torch.Tensor],
+    block_ids: torch.Tensor,
+    key_out: Sequence[torch.Tensor],
+    value_out: Sequence[torch.Tensor],
+) -> None:
+    """``gather_blocks`` from 4-bit pools: whole blocks by block table for every layer, as the bf16 values they stand
+    for (exact), in one launch.
+
+    block_ids: ``[B, nb]`` int64 (rows may be strided); outputs: contiguous ``[B, nb * block_size, H_kv, 128]`` bf16.
+    """
+    num_layers = len(key_pools)
+    if not (len(value_pools) == len(key_out) == len(value_out) == num_layers):
+        raise ValueError("gather_blocks_fp4: per-layer lists differ in length")
+    if num_layers == 0:
+        return
+    pool0 = _require_fp4_pools(key_pools, value_pools)
+    device, index = pool0.device, pool0.get_device()
+    _require_gpu("block_ids", block_ids, device)
+    _require_index("block_ids", block_ids, 2)
+    num_blocks, sub, num_kv_heads, _ = pool0.shape
+    batch, nb = block_ids.shape
+    expect = (batch, nb * sub * KERNEL_BLOCK_SIZE, num_kv_heads, 128)
+    for name, tensors in (("key_out", key_out), ("value_out", value_out)):
+        for t in tensors:
+            if t.get_device() != index:
+                _require_gpu(name, t, device)
+            if t.shape != expect or t.dtype is not torch.bfloat16 or not t.is_contiguous():
+                raise ValueError(f"{name}: expected contiguous {expect} bf16, got {tuple(t.shape)} {t.dtype}")
+    if batch == 0 or nb == 0:
+        return
+    _check_range("block_ids", block_ids, num_blocks)
+    if sub > 1:
+        block_ids, num_blocks, nb = _fp4_sub_block_ids(block_ids, num_blocks, sub), num_blocks * sub, nb * sub
+    if block_ids.stride(1) != 1 or (batch > 1 and block_ids.stride(0) < nb):
+        block_ids = block_ids.contiguous()
+    _call(device, "mi_gather_blocks_fp4", _native.pointer_array([t.data_ptr() for t in key_pools]),
+          _native.pointer_array([t.data_ptr() for t in value_pools]), num_blocks, block_ids.data_ptr(),
+          block_ids.stride(0) if batch > 1 else nb, batch, nb,
+          _native.pointer_array([t.data_ptr() for t in key_out]), _native.pointer_array([t.data_ptr() for t in value_out]),
+          num_layers, num_kv_heads, 128, _stream(device))
+
+
+def paged_decode_fp4_workspace_bytes(batch: int, max_blocks: int, num_heads: int, num_kv_heads: int,
+                                     block_size: int = KERNEL_BLOCK_SIZE) -> int:
+    """Workspace for ``paged_decode_attention_fp4`` on ``[batch, max_blocks]`` tables (0: none needed)."""
+    return int(_native.load().mi_paged_decode_fp4_workspace_bytes(
+        batch, max_blocks * max(block_size // KERNEL_BLOCK_SIZE, 1), num_heads, num_kv_heads))
+
+
+def paged_decode_attention_fp4(
+    query: torch.Tensor,
+    key_pool: torch.Tensor,
+    value_pool: torch.Tensor,
+    block_tables: torch.Tensor,
+    context_lens: torch.Tensor,
+    scale: float,
+    out: torch.Tensor | None = None,
+    workspace: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """``paged_decode_attention`` straight from 4-bit pools (``fp4_pool_shape``).
+
+    query: ``[B, H, 128]`` bf16 (D contiguous), at most 8 query heads per KV head; block_tables ``[B, max_blocks]``
+    int64 (null-padded); context_lens ``[B]`` int64 (includes the new token; 0: a zero row).  Returns ``out``
+    ``[B, H * 128]`` bf16.  ``workspace`` (optional, uint8, reused across calls of one stream) holds the partials of
+    long contexts; it is allocated here when missing or too small.
+    """
+    pool0 = _require_fp4_pools((key_pool,), (value_pool,))
+    device, index = pool0.device, pool0.get_device()
+    for name, t in (("query", query), ("block_tables", block_tables), ("context_lens", context_lens)):
+        if t.get_device() != index:
+            _require_gpu(name, t, device)
+    _require_index("block_tables", block_tables, 2)
+    _require_index("context_lens", context_lens, 1)
+    if query.ndim != 3 or query.dtype is not torch.bfloat16 or query.stride(2) != 1 or query.shape[2] != 128:
+        raise ValueError(f"query must be [B, H, 128] bf16 with D contiguous, got {tuple(query.shape)} {query.dtype}")
+    batch, num_heads, head_dim = query.shape
+    num_blocks, sub, num_kv_heads, _ = pool0.shape
+    if block_tables.shape[0] != batch or context_lens.shape[0] != batch:
+        raise ValueError("block_tables / context_lens batch differs from query batch")
+    if out is None:
+        out = torch.empty((batch, num_heads * head_dim), dtype=torch.bfloat16, device=device)
+    else:
+        _require_gpu("out", out, device)
+        if out.shape != (batch, num_heads * head_dim) or out.dtype is not torch.bfloat16 or out.stride(1) != 1:
+            raise ValueError(f"out must be [B, H * D] bf16 with unit inner stride, got {tuple(out.shape)}")
+    if batch == 0:
+        return out
+    _check_range("block_tables", block_tables, num_blocks)
+    if sub > 1:
+        block_tables, num_blocks = _fp4_sub_block_ids(block_tables, num_blocks, sub), num_blocks * sub
+    max_blocks = block_tables.shape[1]
+    if max_blocks > 0 and (block_tables.stride(1) != 1 or (batch > 1 and block_tables.stride(0) < max_blocks)):
+        block_tables = block_tables.contiguous()
+    if batch > 1 and context_lens.stride(0) <= 0:
+        context_lens = context_lens.contiguous()
+    need = _native.load().mi_paged_decode_fp4_workspace_bytes(batch, max_blocks, num_heads, num_kv_heads)
+    ws_ptr, ws_bytes = None, 0
+    if need > 0:
+        if workspace is None or workspace.numel() * workspace.element_size() < need:
+            workspace = torch.empty(need, dtype=torch.uint8, device=device)
+        elif workspace.get_device() != index or not workspace.is_contiguous():
+            raise ValueError(f"workspace must be contiguous on {device}")
+        ws_ptr, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    _call(device, "mi_paged_decode_attention_fp4", out.data_ptr(), out.stride(0) if batch > 1 else num_heads * head_dim,
+          query.data_ptr(), query.stride(0) if batch > 1 else num_heads * head_dim,
+          query.stride(1) if num_heads > 1 else head_dim, key_pool.data_ptr(), value_pool.data_ptr(), num_blocks,
+          block_tables.data_ptr(), block_tables.stride(0) if batch > 1 else max(max_blocks, 1), max_blocks,
+          context_lens.data_ptr(), context_lens.stride(0) if batch > 1 else 1, batch, num_heads, num_kv_heads, head_dim,
+          float(scale), ws_ptr, ws_bytes, _stream(device))
+    return out
+
+
+def chunked_prefill_attention_fp4(
+    query: torch.Tensor,
+    key: torch.Tensor,
+    value: torch.Tensor,
+    key_pool: torch.Tensor,
+    value_pool: torch.Tensor,
+    history_blocks: torch.Tensor,
+    start_lens: torch.Tensor,
+    chunk_lens: torch.Tensor,
+    scale: float,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """``chunked_prefill_attention`` with the history read from 4-bit pools (``fp4_pool_shape``).
+
+    query ``[B, H, L, 128]``; key / value ``[B, H_kv, L, 128]`` bf16 (left-padded chunk, D contiguous, any other
+    strides); history_blocks ``[B, nb]`` int64 (may have ``nb = 0``); start_lens / chunk_lens ``[B]`` int64.
+    Returns ``out`` ``[B, L, H * 128]`` bf16; left-padding rows are zero.
+    """
+    pool0 = _require_fp4_pools((key_pool,), (value_pool,))
+    device, index = pool0.device, pool0.get_device()
+    for name, t in (("query", query), ("key", key), ("value", value), ("history_blocks", history_blocks),
+                    ("start_lens", start_lens), ("chunk_lens", chunk_lens)):
+        if t.get_device() != index:
+            _require_gpu(name, t, device)
+    _require_index("history_blocks", history_blocks, 2)
+    _require_index("start_lens", start_lens, 1)
+    _require_index("chunk_lens", chunk_lens, 1)
+    for name, t in (("query", query), ("key", key), ("value", value)):
+        if t.ndim != 4 or t.dtype is not torch.bfloat16 or t.stride(3) != 1 or t.shape[3] != 128:
+            raise ValueError(f"{name} must be 4-d bf16 with a contiguous last dim of 128, got {tuple(t.shape)} {t.dtype}")
+    batch, num_heads, padded_len, head_dim = query.shape
+    num_blocks, sub, num_kv_heads, _ = pool0.shape
+    if key.shape != (batch, num_kv_heads, padded_len, head_dim) or value.shape != key.shape:
+        raise ValueError(f"key/value must be [{batch}, {num_kv_heads}, {padded_len}, {head_dim}]")
+    if history_blocks.shape[0] != batch or start_lens.shape[0] != batch or chunk_lens.shape[0] != batch:
+        raise ValueError("history_blocks / start_lens / chunk_lens batch differs from query batch")
+    if out is None:
+        out = torch.empty((batch, padded_len, num_heads * head_dim), dtype=torch.bfloat16, device=device)
+    else:
+        _require_gpu("out", out, device)
+        if out.shape != (batch, padded_len, num_heads * head_dim) or out.dtype is not torch.bfloat16 or out.stride(2) != 1:
+            raise ValueError(f"out must be [B, L, H * D] bf16 with unit inner stride, got {tuple(out.shape)}")
+    if batch == 0 or padded_len == 0:
+        return out
+    _check_range("history_blocks", history_blocks, num_blocks)
+    if sub > 1:
+        history_blocks, num_blocks = _fp4_sub_block_ids(history_blocks, num_blocks, sub), num_blocks * sub
+    nb = history_blocks.shape[1]
+    if nb > 0 and (history_blocks.stride(1) != 1 or (batch > 1 and history_blocks.stride(0) < nb)):
+        history_blocks = history_blocks.contiguous()
+    if batch > 1 and (start_lens.stride(0) != chunk_lens.stride(0) or start_lens.stride(0) <= 0):
+        start_lens, chunk_lens = start_lens.contiguous(), chunk_lens.contiguous()
+    def strides(t):  # of a dim of one element any stride is good
+        return [st if n > 1 else 0 for st, n in zip(t.stride()[:-1], t.shape)]
+
+    _call(device, "mi_chunked_prefill_attention_fp4", out.data_ptr(), *strides(out), query.data_ptr(), *strides(query),
+          key.data_ptr(), *strides(key), value.data_ptr(), *strides(value),
+          key_pool.data_ptr(), value_pool.data_ptr(), num_blocks, history_blocks.data_ptr() if nb else None,
+          (history_blocks.stride(0) if batch > 1 else nb) if nb else 0, nb, start_lens.data_ptr(), chunk_lens.data_ptr(),
+          start_lens.stride(0) if batch > 1 else 1, batch, padded_len, num_heads, num_kv_heads, head_dim, float(scale),
+          _stream(device))
+    return out
