@@ -43,7 +43,9 @@ HIPCC_FLAGS = [
 # Per-source flags.  exact_attention.hip: the fp64 MFMA accumulators of its prefill kernel in
 # ordinary VGPRs (the compiler's default puts them in AGPRs, which at 256 threads per workgroup
 # pushes the kernel to one wavefront per SIMD; in VGPRs the cached form fits four).
+# fp4_decode_attention.hip: the output accumulators, which the vector unit rescales, without moves to and from AGPRs.
 SOURCE_FLAGS = {
+    "fp4_decode_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=true"],
     "exact_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=true"],
 }
 

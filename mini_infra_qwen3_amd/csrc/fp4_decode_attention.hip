@@ -17,20 +17,28 @@
 //    the tokens.  Output tile t takes dim 8 j + t as its column j: a lane ends with eight dims of a head side by side.
 //  * The running maximum is raised only when a score passes it by 2^8 (with the sums scaled alike, exact).
 //
-// Work: a workgroup takes a KV head and a part of a sequence's blocks, its wavefronts every kWaves-th pair of
-// blocks, each with its own softmax state; the states are joined in LDS.  A sequence of several parts leaves
-// partials in the workspace, which a second launch joins.
+// Work, in one of two forms (Plan):
+//  * Parts: a workgroup takes a KV head and a part of a sequence's blocks, its wavefronts every n-th pair of blocks, each
+//    with its own softmax state, joined in LDS.  A sequence of several parts leaves partials for a second launch.
+//  * Streams: the blocks of all sequences, in order, are cut into as many equal ranges as the device holds wavefronts
+//    (per KV head), whatever the lengths; a wavefront walks its range, sequence by sequence.  Sequences that
+//    a range's end cuts leave partials, two a range at most, for the second launch.
 #include "decode_block.h"
 #include "fp4_record.h"
 
 namespace mi {
 namespace {
 
-constexpr int kWaves = 4;
-constexpr int kThreads = 64 * kWaves;
-constexpr int kMaxGroup = 8;        // query heads per KV head
-constexpr int kMaxPartBlocks = 64;  // a lane holds one block id
-constexpr int kMergeThreads = 128;
+constexpr int kMaxGroup = 8;      // query heads per KV head
+// Registers: at most 128 and 168.  The stream form's loop takes 160 with the next sequence's query in them; at four
+// wavefronts a SIMD (128, with spills) the 256-sequence case below took 189 us instead of 154, at two 159.
+constexpr int kPartWavesPerSimd = 4;
+constexpr int kStreamWavesPerSimd = 3;
+constexpr int kIds = 64;          // block ids in a register, one a lane
+constexpr int kStreamWaves = 4;   // wavefronts of a workgroup of the stream form
+constexpr int kMaxStreamBatch = 4096;  // sequences whose prefix sums a workgroup holds in LDS
+constexpr int kMinStreamBlocks = 8;    // blocks of a range at least
+constexpr int kMergeThreads = 256;
 
 struct Fp4DecodeArgs {
   uint16_t* out;
@@ -47,12 +55,18 @@ struct Fp4DecodeArgs {
   int32_t max_blocks;
   int32_t kv_heads;
   int32_t group;
-  int32_t part_blocks;  // blocks of a part
+  int32_t batch;
+  int32_t part_blocks;  // parts form: blocks of a part, at most kIds per wavefront
   int32_t parts;        // parts per sequence
+  int32_t streams;      // streams form: ranges per KV head at most; 0: the parts form
   float scale;          // |scale| log2 e; the queries carry the sign
   uint32_t q_sign;      // 0x80008000 when scale < 0
-  float* ws_acc;        // [batch, heads, parts, 128]
-  float* ws_ml;         // [batch, heads, parts, 2]: max (log2 units) and sum
+  // Partials: accumulators [slots, 128], and [slots, 2] of max (log2 units) and sum.  Parts: slot (b heads + h) parts + part.
+  // Streams: slot 2 stream heads + h for the cut sequence that a range begins with, (2 stream + 1) heads + h for the one
+  // that it ends with; and the sequences' first blocks in the list, [batch + 1].
+  float* ws_acc;
+  float* ws_ml;
+  int32_t* ws_off;
 };
 
 __device__ __forceinline__ int64_t tokens_of(const Fp4DecodeArgs& a, int64_t b) {
@@ -60,42 +74,68 @@ __device__ __forceinline__ int64_t tokens_of(const Fp4DecodeArgs& a, int64_t b) 
   return min(n, static_cast<int64_t>(a.max_blocks) * kFp4Tokens);
 }
 
-struct Piece {  // a lane's part of one block
-  u32x4 k, v;
-  uint32_t ks, vs;
+// A lane's part of two blocks: codes and scale bytes.
+struct Pair {
+  u32x4 k[2], v[2];
+  uint32_t ks[2], vs[2];
 };
 
-// Two blocks (32 tokens from tok_base, those from n on hidden) of one KV head.  st as MfmaState: m of head
-// lane % 8, l the lane's share of its sum, o[t][i]: head 4 (lane / 16) + i (rows 8 .. 15 repeat 0 .. 7), dim 8 (lane % 16) + t.
-__device__ __forceinline__ void attend_pair(MfmaState& st, const i32x8& q, uint32_t q_scale, Piece (&x)[2], float scale,
-                                            int64_t tok_base, int64_t n, int lane) {
-  const int r = lane >> 4;
-  const bool tail = tok_base + 2 * kFp4Tokens > n;  // uniform
-  float s[8];
+__device__ __forceinline__ int blocks_of(int64_t n) {
+  return n <= 0 ? 0 : static_cast<int>((n + kFp4Tokens - 1) / kFp4Tokens);
+}
+
+// The workgroup's queries as B operands of the scaled product, through LDS: thread 32 h + x takes dims 4 x .. 4 x + 3 of
+// head h (zeros past the group).  split_query's numbers, without every wavefront making all of them.
+struct QueryStage {
+  uint32_t codes[2][kMaxGroup][kHeadDim / 4];  // [hi, lo][head]
+  uint32_t scales[2][kMaxGroup];
+};
+__device__ __forceinline__ void stage_queries(QueryStage& s, const Fp4DecodeArgs& a, int64_t b, int g) {
+  const int h = threadIdx.x >> 5, x = threadIdx.x & 31;
+  if (h >= kMaxGroup) return;  // whole wavefronts
+  typedef uint32_t u32x2v __attribute__((ext_vector_type(2)));
+  u32x2v v{};
+  if (h < a.group) {
+    v = *reinterpret_cast<const u32x2v*>(a.query + b * a.q_row + (static_cast<int64_t>(g) * a.group + h) * a.q_head + 4 * x);
+    v[0] ^= a.q_sign;
+    v[1] ^= a.q_sign;
+  }
+  const uint32_t w0 = v[0], w1 = v[1];
+  uint32_t amax = max(max(w0 & 0x7fffu, (w0 >> 16) & 0x7fffu), max(w1 & 0x7fffu, (w1 >> 16) & 0x7fffu));
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) amax = max(amax, static_cast<uint32_t>(__shfl_xor(static_cast<int>(amax), d)));
+  const SplitScale sc(amax);
+  int hi, lo;
+  split4(w0, w1, sc.up, hi, lo);
+  s.codes[0][h][x] = hi;
+  s.codes[1][h][x] = lo;
+  if (x == 0) {
+    s.scales[0][h] = sc.hi;
+    s.scales[1][h] = sc.lo;
+  }
+}
+
+// The raw scores of two blocks: s[4 b + i] of head lane % 8 and token 16 b + 4 (lane / 16) + i.
+__device__ __forceinline__ void pair_scores(float (&s)[8], const i32x8& q, uint32_t q_scale, const Pair& x) {
 #pragma unroll
   for (int b = 0; b < 2; ++b) {
     i32x8 k{};
 #pragma unroll
-    for (int e = 0; e < 4; ++e) k[e] = x[b].k[e];
+    for (int e = 0; e < 4; ++e) k[e] = x.k[b][e];
     f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-    acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, q, acc, 4, 0, 0, x[b].ks, 0, q_scale);
+    acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, q, acc, 4, 0, 0, x.ks[b], 0, q_scale);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) s[4 * b + i] = (acc[i] + dpp_f32<0x128>(acc[i])) * scale;  // row_ror:8
+    for (int i = 0; i < 4; ++i) s[4 * b + i] = acc[i] + dpp_f32<0x128>(acc[i]);  // row_ror:8
   }
-  if (tail) {  // hidden tokens: no weight, and a value of zero whatever their bytes say
-#pragma unroll
-    for (int b = 0; b < 2; ++b)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (tok_base + 16 * b + 4 * r + i >= n) {
-          s[4 * b + i] = -INFINITY;
-          x[b].v[i] = 0;
-          x[b].vs &= ~(0xffu << (8 * i));
-        }
-  }
+}
+
+// Softmax of a pair's scores: the weights as bf16.  st as MfmaState: m of head lane % 8, l the lane's share of its sum,
+// o[t][i]: head 4 (lane / 16) + i (rows 8 .. 15 repeat 0 .. 7), dim 8 (lane % 16) + t.
+__device__ __forceinline__ bf16x8 pair_weights(MfmaState& st, const float (&s)[8], float scale, int r) {
   float mb = s[0];
 #pragma unroll
   for (int e = 1; e < 8; ++e) mb = fmaxf(mb, s[e]);
+  mb *= scale;
   if (__builtin_amdgcn_ballot_w64(mb > st.m + kRescaleSlack) != 0) {
     const float nm = fmaxf(st.m, xmax32(xmax16(mb)));
     const float al = nm == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(st.m - nm);
@@ -111,43 +151,137 @@ __device__ __forceinline__ void attend_pair(MfmaState& st, const i32x8& q, uint3
   const float ref = st.m == -INFINITY ? 0.0f : st.m;
   f32x8 p;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(s[e] - ref);
+  for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], scale, -ref));
   st.l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
-  const bf16x8 pa = __builtin_convertvector(p, bf16x8);
-  u32x4 w[2][4];  // [block][token 4 r + i]: dims 8 j .. 8 j + 7
+  return __builtin_convertvector(p, bf16x8);
+}
+
+// P V of dims 8 j + 2 kPair and the next: eight values of each, unpacked two a convert, paired by token.
+template <int kPair>
+__device__ __forceinline__ void attend_dims(MfmaState& st, const bf16x8& p, const Pair& x, const float (&vs)[2][4]) {
+  uint32_t w[2][4];
 #pragma unroll
   for (int b = 0; b < 2; ++b)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint32_t codes = x[b].v[i];
-      w[b][i] = fp4_unpack8(codes, e8m0_f32((x[b].vs >> (8 * i)) & 0xffu));
+      const uint32_t codes = x.v[b][i];
+      w[b][i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, vs[b][i], kPair));
     }
 #pragma unroll
-  for (int t = 0; t < 8; ++t) {
-    const uint32_t sel = (t & 1) ? 0x07060302u : 0x05040100u;
+  for (int e = 0; e < 2; ++e) {
+    const uint32_t sel = e ? 0x07060302u : 0x05040100u;
     u32x4 f;
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
-      f[2 * b] = __builtin_amdgcn_perm(w[b][1][t >> 1], w[b][0][t >> 1], sel);
-      f[2 * b + 1] = __builtin_amdgcn_perm(w[b][3][t >> 1], w[b][2][t >> 1], sel);
+      f[2 * b] = __builtin_amdgcn_perm(w[b][1], w[b][0], sel);
+      f[2 * b + 1] = __builtin_amdgcn_perm(w[b][3], w[b][2], sel);
     }
-    st.o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(pa, __builtin_bit_cast(bf16x8, f), st.o[t], 0, 0, 0);
+    st.o[2 * kPair + e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(p, __builtin_bit_cast(bf16x8, f), st.o[2 * kPair + e], 0, 0, 0);
   }
 }
+__device__ __forceinline__ void attend_values(MfmaState& st, const bf16x8& p, const Pair& x) {
+  float vs[2][4];
+#pragma unroll
+  for (int b = 0; b < 2; ++b)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) vs[b][i] = e8m0_f32((x.vs[b] >> (8 * i)) & 0xffu);
+  attend_dims<0>(st, p, x, vs);
+  attend_dims<1>(st, p, x, vs);
+  attend_dims<2>(st, p, x, vs);
+  attend_dims<3>(st, p, x, vs);
+}
 
-__global__ __launch_bounds__(kThreads) void fp4_decode_kernel(const Fp4DecodeArgs a) {
+// A wavefront's walk over blocks of one sequence and KV head: the pipeline's registers and addresses.
+typedef const __attribute__((address_space(1))) char* global_t;
+typedef const __attribute__((address_space(1))) u32x4* global4_t;
+struct Walk {
+  Pair x;
+  uint32_t ids;  // block ids, one a lane
+  int64_t block_bytes;
+  const char* k_pool;  // at this KV head
+  const char* v_pool;
+  uint32_t code_off, ks_off, vs_off;
+
+  __device__ __forceinline__ Walk(const Fp4DecodeArgs& a, int g, int lane) {
+    block_bytes = static_cast<int64_t>(a.kv_heads) * kFp4Record;
+    k_pool = a.key_pool + g * kFp4Record;
+    v_pool = a.value_pool + g * kFp4Record;
+    code_off = 16 * lane;
+    ks_off = kFp4Codes + lane;
+    vs_off = kFp4Codes + 16 * (lane >> 4) + 4 * ((lane & 15) >> 2);
+  }
+  // Id of block i of the `count` from row: past the end the last one (which is hidden there), outside the pool the null block.
+  __device__ __forceinline__ static uint32_t fetch_id(const Fp4DecodeArgs& a, const int64_t* row, int count, int i) {
+    const int64_t id = row[min(i, count - 1)];
+    return id < 0 || id >= a.num_blocks ? 0u : static_cast<uint32_t>(id);  // fewer than 2^31 blocks
+  }
+  // Scalar bases and 32-bit lane offsets.
+  __device__ __forceinline__ global_t base_of(const char* pool, int i) const {
+    global_t p = (global_t)(pool + __builtin_amdgcn_readlane(ids, i) * block_bytes);
+    asm("" : "+s"(p));
+    return p;
+  }
+  __device__ __forceinline__ void load_k(int i) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const global_t p = base_of(k_pool, i + e);
+      x.k[e] = __builtin_nontemporal_load((global4_t)(p + code_off));
+      x.ks[e] = *reinterpret_cast<const __attribute__((address_space(1))) uint8_t*>(p + ks_off);
+    }
+  }
+  __device__ __forceinline__ void load_v(int i) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const global_t p = base_of(v_pool, i + e);
+      x.v[e] = __builtin_nontemporal_load((global4_t)(p + code_off));
+      x.vs[e] = *reinterpret_cast<const __attribute__((address_space(1))) uint32_t*>(p + vs_off);
+    }
+  }
+  // The pair in x, `left` tokens of which (32 or more: all) are visible; next(): loads K of the next pair.  A pair's K
+  // registers take the next pair's as soon as its scores are there; its V registers after P V, by the caller.
+  template <typename Next>
+  __device__ __forceinline__ void attend(MfmaState& st, const i32x8& q, uint32_t q_scale, float scale, int64_t left, int r, Next next) {
+    float s[8];
+    pair_scores(s, q, q_scale, x);
+    next();
+    if (left < 2 * kFp4Tokens) {  // uniform.  Hidden tokens: no weight, and a value of zero whatever their bytes say
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (16 * (e >> 2) + 4 * r + (e & 3) >= left) {
+          s[e] = -INFINITY;
+          x.v[e >> 2][e & 3] = 0;
+          x.vs[e >> 2] &= ~(0xffu << (8 * (e & 3)));
+        }
+    }
+    const bf16x8 p = pair_weights(st, s, scale, r);
+    attend_values(st, p, x);
+  }
+};
+
+__device__ __forceinline__ void start(MfmaState& st) {
+  st.m = -INFINITY;
+  st.l = 0.0f;
+#pragma unroll
+  for (int t = 0; t < 8; ++t) st.o[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+}
+
+template <int kWaves>
+__global__ __launch_bounds__(64 * kWaves, kPartWavesPerSimd) void fp4_part_kernel(const Fp4DecodeArgs a) {
   extern __shared__ float s_raw[];  // [kWaves][group][128], then [kWaves][group][2]
+  __shared__ QueryStage s_q;
+  constexpr int kThreads = 64 * kWaves;
+  static_assert(kThreads >= 32 * kMaxGroup, "a thread for every four query elements");
   float* s_ml = s_raw + kWaves * a.group * kHeadDim;
-  const int g = static_cast<int>(blockIdx.x % a.kv_heads);
-  const int64_t unit = blockIdx.x / a.kv_heads;
-  const int64_t b = unit / a.parts;
-  const int part = static_cast<int>(unit % a.parts);
+  const uint32_t unit = blockIdx.x / static_cast<uint32_t>(a.kv_heads);
+  const int g = static_cast<int>(blockIdx.x - unit * a.kv_heads);
+  const int64_t b = unit / static_cast<uint32_t>(a.parts);
+  const int part = static_cast<int>(unit % static_cast<uint32_t>(a.parts));
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
   const int j = lane & 15, r = lane >> 4;
   const int64_t n = tokens_of(a, b);
   uint16_t* out = a.out + b * a.out_row + static_cast<int64_t>(g) * a.group * kHeadDim;
-  const int blocks = n <= 0 ? 0 : static_cast<int>((n + kFp4Tokens - 1) / kFp4Tokens);
+  const int blocks = blocks_of(n);
   const int first = part * a.part_blocks;  // < max_blocks
   if (first >= blocks) {                   // uniform
     if (part == 0)                         // an empty context: zero rows
@@ -155,42 +289,37 @@ __global__ __launch_bounds__(kThreads) void fp4_decode_kernel(const Fp4DecodeArg
     return;
   }
   const int count = min(a.part_blocks, blocks - first);
-  int64_t id = a.block_tables[b * a.bt_stride + first + min(lane, count - 1)];
-  if (id < 0 || id >= a.num_blocks) id = 0;
-  const uint32_t id_lo = static_cast<uint32_t>(id);  // fewer than 2^31 blocks
-  const int c = j & 7;
-  const SplitQuery split = split_query(a.query + b * a.q_row + (static_cast<int64_t>(g) * a.group + min(c, a.group - 1)) * a.q_head,
-                                       c < a.group, a.q_sign, r);
-  const i32x8 q = j < 8 ? split.hi : split.lo;
-  const uint32_t q_scale = j < 8 ? split.hi_scale : split.lo_scale;
+  Walk walk(a, g, lane);
+  // Lanes 2 k and 2 k + 1 hold the ids of the wavefront's k-th pair, blocks 2 w + 2 k kWaves and the next.
+  walk.ids = Walk::fetch_id(a, a.block_tables + b * a.bt_stride + first, count, 2 * w + kWaves * (lane & ~1) + (lane & 1));
   MfmaState st;
-  st.m = -INFINITY;
-  st.l = 0.0f;
-#pragma unroll
-  for (int t = 0; t < 8; ++t) st.o[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  const int64_t block_bytes = static_cast<int64_t>(a.kv_heads) * kFp4Record;
-  auto load = [&](Piece (&x)[2], int i) {  // blocks i, i + 1 of the part; past its end the last one again, which is hidden
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int64_t at = __builtin_amdgcn_readlane(id_lo, min(i + e, count - 1)) * block_bytes + g * kFp4Record;
-      const char* k = a.key_pool + at;
-      const char* v = a.value_pool + at;
-      x[e].k = load_vec<true>(reinterpret_cast<const u32x4*>(k + 16 * lane));
-      x[e].v = load_vec<true>(reinterpret_cast<const u32x4*>(v + 16 * lane));
-      x[e].ks = *reinterpret_cast<const uint8_t*>(k + kFp4Codes + lane);
-      x[e].vs = *reinterpret_cast<const uint32_t*>(v + kFp4Codes + 16 * r + 4 * (j >> 2));
-    }
-  };
+  start(st);
   // The context's end as the part sees it: a pair past the part's own blocks is hidden.
-  const int64_t end = min(n, static_cast<int64_t>(first + count) * kFp4Tokens);
-  Piece x[2][2];
-  if (2 * w < count) load(x[0], 2 * w);
-  for (int i = 2 * w; i < count; i += 4 * kWaves) {
-    if (i + 2 * kWaves < count) load(x[1], i + 2 * kWaves);
-    attend_pair(st, q, q_scale, x[0], a.scale, static_cast<int64_t>(first + i) * kFp4Tokens, end, lane);
-    if (i + 2 * kWaves >= count) break;
-    if (i + 4 * kWaves < count) load(x[0], i + 4 * kWaves);
-    attend_pair(st, q, q_scale, x[1], a.scale, static_cast<int64_t>(first + i + 2 * kWaves) * kFp4Tokens, end, lane);
+  const int64_t end = min(n - static_cast<int64_t>(first) * kFp4Tokens, static_cast<int64_t>(count) * kFp4Tokens);
+  int i = 2 * w;
+  if (i < count) {
+    walk.load_k(0);
+    walk.load_v(0);
+  }
+  stage_queries(s_q, a, b, g);
+  __syncthreads();
+  i32x8 q;
+  {
+    const u32x4 lo = *reinterpret_cast<const u32x4*>(&s_q.codes[j >> 3][j & 7][4 * r]);
+    const u32x4 hi = *reinterpret_cast<const u32x4*>(&s_q.codes[j >> 3][j & 7][16 + 4 * r]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      q[e] = lo[e];
+      q[4 + e] = hi[e];
+    }
+  }
+  const uint32_t q_scale = s_q.scales[j >> 3][j & 7];
+  for (int k = 2; i < count; i += 2 * kWaves, k += 2) {
+    const bool more = i + 2 * kWaves < count;
+    walk.attend(st, q, q_scale, a.scale, end - static_cast<int64_t>(i) * kFp4Tokens, r, [&] {
+      if (more) walk.load_k(k);
+    });
+    if (more) walk.load_v(k);
   }
   const float l = xsum32_f32(xsum16_f32(st.l));  // lane: head lane % 8
 #pragma unroll
@@ -233,33 +362,266 @@ __global__ __launch_bounds__(kThreads) void fp4_decode_kernel(const Fp4DecodeArg
   }
 }
 
-// Joins the parts of the sequences that have several: one workgroup per sequence and head, a thread per dim.
-__global__ __launch_bounds__(kMergeThreads) void fp4_merge_kernel(const Fp4DecodeArgs a) {
-  const int64_t heads = static_cast<int64_t>(a.kv_heads) * a.group;
-  const int64_t b = blockIdx.x / heads, h = blockIdx.x % heads;
-  const int64_t n = tokens_of(a, b);
-  const int blocks = n <= 0 ? 0 : static_cast<int>((n + kFp4Tokens - 1) / kFp4Tokens);
-  if (blocks <= a.part_blocks) return;
-  const int parts = (blocks + a.part_blocks - 1) / a.part_blocks;
-  const int64_t at = (b * heads + h) * a.parts;
-  float M = -INFINITY;
-  for (int p = 0; p < parts; ++p) M = fmaxf(M, a.ws_ml[2 * (at + p)]);
-  float L = 0.0f, o = 0.0f;
-  for (int p = 0; p < parts; ++p) {
-    const float m = a.ws_ml[2 * (at + p)];
-    const float e = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - M);
-    L += e * a.ws_ml[2 * (at + p) + 1];
-    o += e * a.ws_acc[(at + p) * kHeadDim + threadIdx.x];
+// The cut of `total` > 0 blocks into ranges, none empty: range s begins at s q + min(s, rem).
+struct Cut {
+  int count, q, rem;
+  __device__ __forceinline__ Cut(int total, int streams) {
+    count = max(min(streams, (total + kMinStreamBlocks - 1) / kMinStreamBlocks), 1);
+    q = total / count;
+    rem = total - q * count;
   }
-  a.out[b * a.out_row + h * kHeadDim + threadIdx.x] = static_cast<uint16_t>(f32_to_bf16_bits(o / L));
+  __device__ __forceinline__ int begin(int s) const { return s * q + min(s, rem); }
+  __device__ __forceinline__ int of(int x) const {  // the range that holds block x
+    const int wide = rem * (q + 1);
+    return x < wide ? x / (q + 1) : rem + (x - wide) / q;
+  }
+};
+
+__global__ __launch_bounds__(64 * kStreamWaves, kStreamWavesPerSimd) void fp4_stream_kernel(const Fp4DecodeArgs a) {
+  extern __shared__ int s_off[];  // [batch + 1]: the sequences' first blocks in the list
+  __shared__ int s_wave[kStreamWaves];
+  constexpr int kThreads = 64 * kStreamWaves;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  int carry = 0;
+  for (int base = 0; base < a.batch; base += kThreads) {
+    const int b = base + threadIdx.x;
+    int v = b < a.batch ? blocks_of(tokens_of(a, b)) : 0;
+    for (int d = 1; d < 64; d <<= 1) {
+      const int y = __shfl_up(v, d);
+      if (lane >= d) v += y;
+    }
+    if (lane == 63) s_wave[w] = v;
+    __syncthreads();
+    int before = carry;
+#pragma unroll
+    for (int k = 0; k < kStreamWaves; ++k) {
+      before += k < w ? s_wave[k] : 0;
+      carry += s_wave[k];
+    }
+    if (b < a.batch) s_off[b + 1] = before + v;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) s_off[0] = 0;
+  __syncthreads();
+  const int total = carry;
+  if (blockIdx.x == 0)
+    for (int b = threadIdx.x; b <= a.batch; b += kThreads) a.ws_off[b] = s_off[b];
+  if (total == 0) return;
+  const Cut cut(total, a.streams);
+  const int id = static_cast<int>(blockIdx.x) * kStreamWaves + w;  // consecutive wavefronts: the KV heads of a range
+  const int stream = __builtin_amdgcn_readfirstlane(id / a.kv_heads);
+  const int g = __builtin_amdgcn_readfirstlane(id % a.kv_heads);
+  if (stream >= cut.count) return;
+  const int begin = __builtin_amdgcn_readfirstlane(cut.begin(stream)), end = __builtin_amdgcn_readfirstlane(cut.begin(stream + 1));
+  int b = 0;
+  for (int hi = a.batch; hi - b > 1;) {  // s_off[b] <= begin < s_off[hi]
+    const int mid = (b + hi) >> 1;
+    if (s_off[mid] <= begin) b = mid; else hi = mid;
+  }
+  b = __builtin_amdgcn_readfirstlane(b);
+  const int j = lane & 15, r = lane >> 4;
+  const int64_t heads = static_cast<int64_t>(a.kv_heads) * a.group;
+  // The range's blocks of one sequence; the next one's ids, query and first blocks are on their way before it ends.
+  struct Segment {
+    int b, at, first, count;  // sequence; first block in the list and in the sequence; blocks
+    bool whole;
+  };
+  auto segment_at = [&](int b, int at) __attribute__((always_inline)) {
+    while (s_off[b + 1] <= at) ++b;  // empty contexts
+    b = __builtin_amdgcn_readfirstlane(b);
+    const int seq0 = __builtin_amdgcn_readfirstlane(s_off[b]), seq1 = __builtin_amdgcn_readfirstlane(s_off[b + 1]);
+    return Segment{b, at, at - seq0, min(end, seq1) - at, at == seq0 && seq1 <= end};
+  };
+  auto row_of = [&](const Segment& x) __attribute__((always_inline)) { return a.block_tables + x.b * a.bt_stride + x.first; };
+  const int qh = min(j & 7, a.group - 1);
+  const uint16_t* q_head = a.query + (static_cast<int64_t>(g) * a.group + qh) * a.q_head;
+  const bool q_live = (j & 7) < a.group;
+  Walk walk(a, g, lane);
+  QueryWords words;
+  Segment seg = segment_at(b, begin);
+  walk.ids = Walk::fetch_id(a, row_of(seg), seg.count, lane);
+  words.load(q_head + seg.b * a.q_row, q_live, a.q_sign, r);
+  walk.load_k(0);
+  walk.load_v(0);
+  for (;;) {
+    const int64_t* row = row_of(seg);
+    const int count = seg.count;
+    uint32_t ids_next = count > kIds ? Walk::fetch_id(a, row + kIds, count - kIds, lane) : 0u;
+    i32x8 q;
+    const SplitScale split = split_query(words, [&](int i, int hi, int lo) { q[i] = j < 8 ? hi : lo; });
+    const uint32_t q_scale = j < 8 ? split.hi : split.lo;
+    const bool another = seg.at + count < end;
+    Segment next_seg = seg;
+    uint32_t ids_ahead = 0;
+    if (another) {
+      next_seg = segment_at(seg.b + 1, seg.at + count);
+      ids_ahead = Walk::fetch_id(a, row_of(next_seg), next_seg.count, lane);
+      words.load(q_head + next_seg.b * a.q_row, q_live, a.q_sign, r);
+    }
+    const int64_t visible = min(tokens_of(a, seg.b) - static_cast<int64_t>(seg.first) * kFp4Tokens, static_cast<int64_t>(count) * kFp4Tokens);
+    MfmaState st;
+    start(st);
+    for (int i = 0, ahead = 2; i < count; i += 2, ahead += 2) {  // ahead: the next pair's place in the window of ids
+      bool more = true;
+      if (i + 2 >= count) {
+        more = another;
+        ahead = 0;
+        walk.ids = ids_ahead;
+      } else if (ahead == kIds) {
+        ahead = 0;
+        walk.ids = ids_next;
+        if (count - i - 2 > kIds) ids_next = Walk::fetch_id(a, row + i + 2 + kIds, count - i - 2 - kIds, lane);
+      }
+      walk.attend(st, q, q_scale, a.scale, visible - static_cast<int64_t>(i) * kFp4Tokens, r, [&] {
+        if (more) walk.load_k(ahead);
+      });
+      if (more) walk.load_v(ahead);
+    }
+    const float l = xsum32_f32(xsum16_f32(st.l));
+    uint16_t* out = a.out + seg.b * a.out_row + static_cast<int64_t>(g) * a.group * kHeadDim + 8 * j;
+    const int64_t slot = (2 * static_cast<int64_t>(stream) + (seg.at == begin ? 0 : 1)) * heads + static_cast<int64_t>(g) * a.group;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int h = 4 * r + i;
+      const float lh = __shfl(l, h & 7), mh = __shfl(st.m, h & 7);
+      if (h >= a.group) continue;
+      const float o[8] = {st.o[0][i], st.o[1][i], st.o[2][i], st.o[3][i], st.o[4][i], st.o[5][i], st.o[6][i], st.o[7][i]};
+      if (seg.whole) {
+        store_bf16x8(out + h * kHeadDim, o, 1.0f / lh);
+      } else {
+        float4* dst = reinterpret_cast<float4*>(a.ws_acc + (slot + h) * kHeadDim + 8 * j);
+        dst[0] = make_float4(o[0], o[1], o[2], o[3]);
+        dst[1] = make_float4(o[4], o[5], o[6], o[7]);
+        if (j == 0) *reinterpret_cast<float2*>(a.ws_ml + 2 * (slot + h)) = make_float2(mh, lh);
+      }
+    }
+    if (!another) return;
+    seg = next_seg;
+  }
 }
 
-// Blocks of a part: enough parts for every CU to have several workgroups, at most a lane's ids.
-int part_blocks_for(int32_t batch, int32_t max_blocks, int32_t num_kv_heads) {
-  const int64_t units = static_cast<int64_t>(batch) * num_kv_heads * max_blocks;
-  int64_t part = units / (4 * static_cast<int64_t>(device_cus()));
-  part = part < 2 * kWaves ? 2 * kWaves : (part > kMaxPartBlocks ? kMaxPartBlocks : part);
-  return static_cast<int>(part / (2 * kWaves) * (2 * kWaves));
+// Joins the partials of cut sequences (and writes the streams form's zero rows): one workgroup per sequence and head, 32
+// threads with four dims each for every kMergeLanes-th partial.
+__global__ __launch_bounds__(kMergeThreads) void fp4_merge_kernel(const Fp4DecodeArgs a) {
+  constexpr int kMergeLanes = kMergeThreads / 32, kMergeWaves = kMergeThreads / 64;
+  __shared__ float s_o[kMergeLanes][kHeadDim], s_l[kMergeLanes], s_m[kMergeWaves];
+  const uint32_t heads = a.kv_heads * a.group;
+  const int64_t b = blockIdx.x / heads, h = blockIdx.x % heads;
+  uint16_t* out = a.out + b * a.out_row + h * kHeadDim;
+  // Partial p is in slot `first` for p = 0, slot at + p step for the others.
+  int64_t first, at, step;
+  int parts;
+  if (a.streams) {
+    const int x0 = a.ws_off[b], x1 = a.ws_off[b + 1];
+    if (x0 == x1) {
+      if (threadIdx.x < kHeadDim) out[threadIdx.x] = 0;
+      return;
+    }
+    const Cut cut(a.ws_off[a.batch], a.streams);
+    const int s0 = cut.of(x0);
+    parts = cut.of(x1 - 1) - s0 + 1;
+    at = 2 * static_cast<int64_t>(s0) * heads + h;
+    step = 2 * static_cast<int64_t>(heads);
+    first = at + (cut.begin(s0) == x0 ? 0 : heads);  // the second slot, unless its range begins with this sequence
+  } else {
+    parts = (blocks_of(tokens_of(a, b)) + a.part_blocks - 1) / a.part_blocks;
+    first = at = (b * heads + h) * a.parts;
+    step = 1;
+  }
+  if (parts <= 1) return;  // written whole
+  const auto slot = [&](int p) { return p == 0 ? first : at + p * step; };
+  float M = -INFINITY;
+  for (int p = threadIdx.x; p < parts; p += kMergeThreads) M = fmaxf(M, a.ws_ml[2 * slot(p)]);
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) M = fmaxf(M, __shfl_xor(M, d));
+  if ((threadIdx.x & 63) == 0) s_m[threadIdx.x >> 6] = M;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kMergeWaves; ++w) M = fmaxf(M, s_m[w]);
+  const int lane = threadIdx.x >> 5, x = threadIdx.x & 31;
+  float L = 0.0f;
+  f32x4 o{};
+  for (int p = lane; p < parts; p += kMergeLanes) {
+    const int64_t at_p = slot(p);
+    const float2 ml = *reinterpret_cast<const float2*>(a.ws_ml + 2 * at_p);
+    const f32x4 v = *reinterpret_cast<const f32x4*>(a.ws_acc + at_p * kHeadDim + 4 * x);
+    // A partial without a visible score has no sums, except where every score was NaN: then its sum is.
+    const float e = ml.x == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(ml.x - M);
+    L += e * ml.y;
+    o += e * v;
+  }
+  *reinterpret_cast<f32x4*>(&s_o[lane][4 * x]) = o;
+  if (x == 0) s_l[lane] = L;
+  __syncthreads();
+  if (threadIdx.x >= kHeadDim) return;
+  L = 0.0f;
+  float sum = 0.0f;
+#pragma unroll
+  for (int k = 0; k < kMergeLanes; ++k) {
+    L += s_l[k];
+    sum += s_o[k][threadIdx.x];
+  }
+  out[threadIdx.x] = static_cast<uint16_t>(f32_to_bf16_bits(sum / L));
+}
+
+// How a launch is cut, and the workspace that takes, by the (sequence, KV head) pairs P, the table's blocks M and their
+// product (context lengths are on the device).  Measured, us a call (16 query / 8 KV heads but where noted; lengths in
+// tokens, M their longest's blocks), whole sequences by 4 / by 8 wavefronts, parts of 16 / 32 / 64 blocks, streams:
+//   whole, 8 wavefronts to 2 P a CU, then 4: a second launch and its joining cost 4 to 5 us, more than short tables' tail
+//       1 x 417             M 27    P 8      6.7 /  6.9     8.4 /   6.6 /   6.7    10.4
+//       8 x 32..1150           72      64   10.7 /  9.4    10.2 /  11.2 /  14.0    14.5
+//      64 x 32..1150           72     512   16.2 / 14.2    20.4 /  19.5 /  22.5    21.6
+//     128 x 32..1150           72    1024   21.9 / 24.8    31.2 /  27.6 /  36.4    29.1
+//    1000 x 32..1150           72    8000    124 /  154     187 /   163 /   206     144
+//      64 x 50..3500          219     512   38.4 / 30.9    39.3 /  32.8 /  42.1    33.4
+//   parts: few pairs
+//       1 x 4000              250       8   17.1 / 19.0     8.8 /   9.7 /  12.1    11.6
+//      16 x 1000..2000        125     128   19.2 / 13.8    13.5 /  13.5 /  15.6    17.9
+//       1 x 65000            4063       8           -      31.3 /  22.9 /  22.6    35.7
+//       4 x 20000..40000     2500      32           -      40.0 /  32.0 /  29.8    35.2
+//      21 x 256..8192, 64 query heads  512  168     -      30.2 /  25.9 /  26.5    29.1
+//   streams: long tables of many pairs, mostly empty
+//      30 x 256..8192         512     240           -      35.0 /  30.9 /  32.5    29.9
+//     100 x 256..8192         512     800           -      90.4 /  79.6 /  80.3    65.6
+//     256 x 256..8192         512    2048           -         - /     - /   254     154
+struct Plan {
+  int32_t streams, part_blocks, parts, waves;
+  int64_t slots, bytes;
+  Plan(int32_t batch, int32_t max_blocks, int32_t num_heads, int32_t num_kv_heads) {
+    const int64_t cus = device_cus();
+    const int64_t pairs = static_cast<int64_t>(batch) * num_kv_heads;
+    const int64_t units = pairs * max_blocks;
+    streams = 0;
+    parts = 1;
+    waves = pairs <= 2 * cus ? 8 : 4;
+    part_blocks = max_blocks > 0 ? max_blocks : 1;
+    slots = bytes = 0;
+    if (max_blocks <= (pairs >= cus ? 4 * kIds : 80)) return;  // whole: every wavefront's ids fit its lanes
+    waves = 4;
+    if (batch <= kMaxStreamBatch && units >= 120000 && static_cast<int64_t>(batch) * max_blocks < (int64_t{1} << 30)) {
+      const int64_t s = cus * 4 * kStreamWavesPerSimd / num_kv_heads;
+      streams = static_cast<int32_t>(s < 1 ? 1 : s);
+      slots = 2 * static_cast<int64_t>(streams) * num_heads;
+      bytes = slots * (kHeadDim + 2) * 4 + (static_cast<int64_t>(batch) + 1) * 4;
+      return;
+    }
+    const int64_t part = (units / 1024 + 7) / 8 * 8;
+    part_blocks = static_cast<int32_t>(part < 16 ? 16 : (part > 64 ? 64 : part));
+    parts = (max_blocks + part_blocks - 1) / part_blocks;
+    if (parts == 1) return;
+    slots = static_cast<int64_t>(batch) * num_heads * parts;
+    bytes = slots * (kHeadDim + 2) * 4;
+  }
+};
+
+template <int kWaves>
+int32_t launch_parts(const char* name, const Fp4DecodeArgs& a, hipStream_t s) {
+  const int64_t groups = static_cast<int64_t>(a.batch) * a.kv_heads * a.parts;
+  if (groups > 0xffffffffll / (64 * kWaves)) return fail(MI_ERR_UNSUPPORTED, "%s: too many workgroups", name);
+  const size_t lds = sizeof(float) * kWaves * a.group * (kHeadDim + 2);
+  fp4_part_kernel<kWaves><<<static_cast<uint32_t>(groups), 64 * kWaves, lds, s>>>(a);
+  return check_launch(name);
 }
 
 }  // namespace
@@ -269,10 +631,7 @@ extern "C" int64_t mi_paged_decode_fp4_workspace_bytes(int32_t batch, int32_t ma
                                                        int32_t num_kv_heads) {
   using namespace mi;
   if (batch <= 0 || max_blocks <= 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0) return 0;
-  const int part = part_blocks_for(batch, max_blocks, num_kv_heads);
-  const int64_t parts = (max_blocks + part - 1) / part;
-  if (parts == 1) return 0;
-  return static_cast<int64_t>(batch) * num_heads * parts * (kHeadDim + 2) * static_cast<int64_t>(sizeof(float));
+  return Plan(batch, max_blocks, num_heads, num_kv_heads).bytes;
 }
 
 extern "C" int32_t mi_paged_decode_attention_fp4(void* out, int64_t out_row_stride, const void* query,
@@ -305,7 +664,8 @@ extern "C" int32_t mi_paged_decode_attention_fp4(void* out, int64_t out_row_stri
   if (num_blocks > 0x7fffffff) return fail(MI_ERR_UNSUPPORTED, "%s: pool too large", name);
   const float c = scale * kLog2e;
   if (!(c == c) || c - c != 0.0f) return fail(MI_ERR_INVALID_ARGUMENT, "%s: scale must be finite", name);
-  const int64_t need = mi_paged_decode_fp4_workspace_bytes(batch, max_blocks, num_heads, num_kv_heads);
+  const Plan plan(batch, max_blocks, num_heads, num_kv_heads);
+  const int64_t need = plan.bytes;
   if (need > 0 && (!workspace || workspace_bytes < need))
     return fail(MI_ERR_WORKSPACE, "%s: workspace of %lld bytes needed, got %lld", name, static_cast<long long>(need),
                 static_cast<long long>(workspace_bytes));
@@ -327,24 +687,30 @@ extern "C" int32_t mi_paged_decode_attention_fp4(void* out, int64_t out_row_stri
   a.max_blocks = max_blocks;
   a.kv_heads = num_kv_heads;
   a.group = group;
-  a.part_blocks = part_blocks_for(batch, max_blocks, num_kv_heads);
-  a.parts = max_blocks > 0 ? (max_blocks + a.part_blocks - 1) / a.part_blocks : 1;
+  a.batch = batch;
+  a.part_blocks = plan.part_blocks;
+  a.parts = plan.parts;
+  a.streams = plan.streams;
   a.scale = c < 0.0f ? -c : c;
   a.q_sign = c < 0.0f ? 0x80008000u : 0u;
   // A scale of zero (every weight alike) still has to leave hidden scores at -inf.
   if (a.scale < 1e-37f) a.scale = 1e-37f;
-  if (a.parts > 1) {
+  if (need > 0) {
     a.ws_acc = static_cast<float*>(workspace);
-    a.ws_ml = a.ws_acc + static_cast<int64_t>(batch) * num_heads * a.parts * kHeadDim;
+    a.ws_ml = a.ws_acc + plan.slots * kHeadDim;
+    a.ws_off = reinterpret_cast<int32_t*>(a.ws_ml + plan.slots * 2);
   }
-  const int64_t groups = static_cast<int64_t>(batch) * num_kv_heads * a.parts;
-  if (groups > 0xffffffffll / kThreads || static_cast<int64_t>(batch) * num_heads > 0xffffffffll / kMergeThreads)
+  if (static_cast<int64_t>(batch) * num_heads > 0xffffffffll / kMergeThreads)
     return fail(MI_ERR_UNSUPPORTED, "%s: too many workgroups", name);
   hipStream_t s = as_stream(stream);
-  const size_t lds = sizeof(float) * kWaves * group * (kHeadDim + 2);
-  fp4_decode_kernel<<<static_cast<uint32_t>(groups), kThreads, lds, s>>>(a);
-  if (const int32_t rc = check_launch(name)) return rc;
-  if (a.parts > 1) {
+  if (a.streams) {
+    const uint32_t groups = static_cast<uint32_t>((static_cast<int64_t>(a.streams) * num_kv_heads + kStreamWaves - 1) / kStreamWaves);
+    fp4_stream_kernel<<<groups, 64 * kStreamWaves, sizeof(int) * (batch + 1), s>>>(a);
+    if (const int32_t rc = check_launch(name)) return rc;
+  } else if (const int32_t rc = plan.waves == 8 ? launch_parts<8>(name, a, s) : launch_parts<4>(name, a, s)) {
+    return rc;
+  }
+  if (need > 0) {
     fp4_merge_kernel<<<static_cast<uint32_t>(batch * num_heads), kMergeThreads, 0, s>>>(a);
     if (const int32_t rc = check_launch(name)) return rc;
   }

@@ -305,11 +305,19 @@ __global__ __launch_bounds__(S::kThreads, 2) void fp4_prefill_kernel(const Fp4Pr
         *reinterpret_cast<u32x4*>(vt + row * 256 + ((octet ^ (row & 15)) * 16)) = fp4_unpack8(codes, e8m0_f32(s));
       }
     };
-    SplitQuery q[kNt];
+    i32x8 q_hi[kNt], q_lo[kNt];
+    uint32_t hi_scale[kNt], lo_scale[kNt];
 #pragma unroll
     for (int nt = 0; nt < kNt; ++nt) {
       const int qi = qw0 + 16 * nt + ql;
-      q[nt] = split_query(q_rows + static_cast<int64_t>(min(qi, L - 1)) * a.q_tok, qi < L && qi >= pad, a.q_sign, gq);
+      QueryWords words;
+      words.load(q_rows + static_cast<int64_t>(min(qi, L - 1)) * a.q_tok, qi < L && qi >= pad, a.q_sign, gq);
+      const SplitScale split = split_query(words, [&](int i, int hi, int lo) {
+        q_hi[nt][i] = hi;
+        q_lo[nt][i] = lo;
+      });
+      hi_scale[nt] = split.hi;
+      lo_scale[nt] = split.lo;
     }
     if (wk < n_hist) {
       load(wk);
@@ -333,9 +341,9 @@ __global__ __launch_bounds__(S::kThreads, 2) void fp4_prefill_kernel(const Fp4Pr
 #pragma unroll
           for (int nt = 0; nt < kNt; ++nt) {
             f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-            acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(kf, q[nt].lo, acc, 4, 0, 0, sc, 0, q[nt].lo_scale);
+            acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(kf, q_lo[nt], acc, 4, 0, 0, sc, 0, lo_scale[nt]);
             sacc[mt][nt] =
-                __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(kf, q[nt].hi, acc, 4, 0, 0, sc, 0, q[nt].hi_scale);
+                __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(kf, q_hi[nt], acc, 4, 0, 0, sc, 0, hi_scale[nt]);
           }
         }
         tile_softmax(t * kKTile, true, (t + 1) * kKTile > nh || rows_edge);

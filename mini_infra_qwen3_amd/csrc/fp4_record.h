@@ -73,46 +73,58 @@ __device__ __forceinline__ int fp4_scale_at(bool value, int t, int j) {
 // hi is in [128, 256), so an element is exact down to 2^-14 of the largest, and off by at most 2^-23 of it below.
 // An infinity or NaN makes both scales NaN, and with them every score.
 typedef int i32x8 __attribute__((ext_vector_type(8)));
-struct SplitQuery {
-  i32x8 hi, lo;
-  uint32_t hi_scale, lo_scale;
-};
-// q: the head's 128 elements (16-byte aligned; not read when !live: zeros), signs flipped by `flip` (0x80008000 or 0).
-// Every lane of the wavefront must be active; the four lanes of a column (lane % 16) hold the same query.
-__device__ __forceinline__ SplitQuery split_query(const uint16_t* q, bool live, uint32_t flip, int r) {
-  uint32_t w[16];
-#pragma unroll
-  for (int p = 0; p < 4; ++p) {
-    const u32x4 v = live ? *reinterpret_cast<const u32x4*>(q + 64 * (p >> 1) + 16 * r + 8 * (p & 1)) : u32x4{};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) w[4 * p + e] = v[e] ^ flip;
+struct SplitScale {
+  float up;         // 2^-s: brings the largest element to [128, 256)
+  uint32_t hi, lo;  // scale codes
+  // amax: the largest magnitude's bf16 bits.  Below 2^-103 the scale stays (up and lo's code in range; elements sink).
+  __device__ __forceinline__ explicit SplitScale(uint32_t amax) {
+    const int e = max(static_cast<int>(amax >> 7), 24);
+    up = __uint_as_float(static_cast<uint32_t>(2 * 127 + 7 - e) << 23);
+    const bool finite = amax < 0x7f80u;
+    hi = finite ? static_cast<uint32_t>(e - 7) : kFp4NanScale;
+    lo = finite ? static_cast<uint32_t>(e - 11) : kFp4NanScale;
   }
+};
+// Four elements (two bf16 pairs) as four hi and four lo codes.
+__device__ __forceinline__ void split4(uint32_t w0, uint32_t w1, float up, int& hi, int& lo) {
+  const float x0 = bf16_lo(w0) * up, x1 = bf16_hi(w0) * up, x2 = bf16_lo(w1) * up, x3 = bf16_hi(w1) * up;
+  hi = __builtin_amdgcn_cvt_pk_fp8_f32(x0, x1, 0, false);
+  hi = __builtin_amdgcn_cvt_pk_fp8_f32(x2, x3, hi, true);
+  const float r0 = x0 - __builtin_amdgcn_cvt_f32_fp8(hi, 0), r1 = x1 - __builtin_amdgcn_cvt_f32_fp8(hi, 1);
+  const float r2 = x2 - __builtin_amdgcn_cvt_f32_fp8(hi, 2), r3 = x3 - __builtin_amdgcn_cvt_f32_fp8(hi, 3);
+  lo = __builtin_amdgcn_cvt_pk_fp8_f32(r0 * 16.0f, r1 * 16.0f, 0, false);
+  lo = __builtin_amdgcn_cvt_pk_fp8_f32(r2 * 16.0f, r3 * 16.0f, lo, true);
+}
+// Lane quad r's part of a head's 128 elements (16-byte aligned; not read when !live: zeros), signs flipped by `flip`
+// (0x80008000 or 0).
+struct QueryWords {
+  uint32_t w[16];
+  __device__ __forceinline__ void load(const uint16_t* q, bool live, uint32_t flip, int r) {
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+      const u32x4 v = live ? *reinterpret_cast<const u32x4*>(q + 64 * (p >> 1) + 16 * r + 8 * (p & 1)) : u32x4{};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[4 * p + e] = v[e] ^ flip;
+    }
+  }
+};
+// put(i, hi, lo) for a lane's code words i = 0 .. 7; returns the scales.  Every lane of the wavefront must be active; the four
+// lanes of a column (lane % 16) hold the same query.
+template <typename Put>
+__device__ __forceinline__ SplitScale split_query(const QueryWords& q, Put put) {
   uint32_t amax = 0;
 #pragma unroll
-  for (int e = 0; e < 16; ++e) amax = max(amax, max(w[e] & 0x7fffu, (w[e] >> 16) & 0x7fffu));
+  for (int e = 0; e < 16; ++e) amax = max(amax, max(q.w[e] & 0x7fffu, (q.w[e] >> 16) & 0x7fffu));
   amax = max(amax, static_cast<uint32_t>(__shfl_xor(static_cast<int>(amax), 16)));
   amax = max(amax, static_cast<uint32_t>(__shfl_xor(static_cast<int>(amax), 32)));
-  // Its exponent field, from 24 up (2^-103: the factor below and lo's scale stay in range; smaller elements sink).
-  const int e = max(static_cast<int>(amax >> 7), 24);
-  const float up = __uint_as_float(static_cast<uint32_t>(2 * 127 + 7 - e) << 23);
-  const bool finite = amax < 0x7f80u;
-  SplitQuery x;
-  x.hi_scale = finite ? static_cast<uint32_t>(e - 7) : kFp4NanScale;
-  x.lo_scale = finite ? static_cast<uint32_t>(e - 11) : kFp4NanScale;
+  const SplitScale s(amax);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {  // four dims each
-    const float x0 = bf16_lo(w[2 * i]) * up, x1 = bf16_hi(w[2 * i]) * up;
-    const float x2 = bf16_lo(w[2 * i + 1]) * up, x3 = bf16_hi(w[2 * i + 1]) * up;
-    int h = __builtin_amdgcn_cvt_pk_fp8_f32(x0, x1, 0, false);
-    h = __builtin_amdgcn_cvt_pk_fp8_f32(x2, x3, h, true);
-    const float r0 = (x0 - __builtin_amdgcn_cvt_f32_fp8(h, 0)) * 16.0f, r1 = (x1 - __builtin_amdgcn_cvt_f32_fp8(h, 1)) * 16.0f;
-    const float r2 = (x2 - __builtin_amdgcn_cvt_f32_fp8(h, 2)) * 16.0f, r3 = (x3 - __builtin_amdgcn_cvt_f32_fp8(h, 3)) * 16.0f;
-    int l = __builtin_amdgcn_cvt_pk_fp8_f32(r0, r1, 0, false);
-    l = __builtin_amdgcn_cvt_pk_fp8_f32(r2, r3, l, true);
-    x.hi[i] = h;
-    x.lo[i] = l;
+  for (int i = 0; i < 8; ++i) {
+    int hi, lo;
+    split4(q.w[2 * i], q.w[2 * i + 1], s.up, hi, lo);
+    put(i, hi, lo);
   }
-  return x;
+  return s;
 }
 
 }  // namespace

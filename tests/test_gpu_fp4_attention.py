@@ -86,6 +86,63 @@ def test_decode_batch_of_many_lengths(native_lib, device):
     check_decode(run_decode(device, *case, contexts), *case, contexts)
 
 
+@pytest.mark.parametrize("heads,kv_heads,batch,width", [
+    (4, 2, 5, 60),       # whole sequences by 8 wavefronts (few pairs, short tables)
+    (2, 2, 300, 100),    # whole by 4 (many pairs)
+    (16, 8, 3, 900),     # parts
+    (4, 2, 50, 1300),    # streams
+    (64, 8, 40, 400),    # streams, 8 heads a group
+    (5, 1, 130, 1000),
+    (9, 3, 60, 700)])
+def test_decode_forms(native_lib, device, heads, kv_heads, batch, width):
+    """Tables wider than any context, so that each way of cutting the work sees short, empty and odd sequences."""
+    rng = np.random.default_rng(batch)
+    contexts = [int(x) for x in rng.integers(0, 330, batch)]
+    contexts[0], contexts[-1], contexts[batch // 2] = 1, 0, 16 * min(width, 70)
+    case = decode_case(batch, contexts, heads, kv_heads, width=width)
+    check_decode(run_decode(device, *case, contexts), *case, contexts)
+    if batch > 2:  # all but one empty; all empty
+        few = [0] * batch
+        check_decode(run_decode(device, *case, few), *case, few)
+        few[batch // 2] = contexts[batch // 2]
+        check_decode(run_decode(device, *case, few), *case, few)
+
+
+def test_decode_long_ranges(native_lib, device):
+    """Enough blocks for every range of the stream form to hold more than 64; against the values read back, in fp64."""
+    contexts = [90000, 5, 70001, 0, 120000, 33333, 100000, 16]
+    kv_heads, heads = 8, 16
+    gen = torch.Generator(device=device).manual_seed(5)
+    need = [-(-n // 16) for n in contexts]
+    num_blocks = 1 + sum(need)
+    kp, vp = (torch.randint(0, 256, data_plane.fp4_pool_shape(num_blocks, 16, kv_heads), generator=gen, device=device,
+                            dtype=torch.uint8) for _ in range(2))
+    for p in (kp, vp):
+        p[..., 1024:] = p[..., 1024:] % 8 + 122
+    perm = torch.randperm(num_blocks - 1, generator=gen, device=device) + 1
+    table = torch.zeros(len(contexts), max(need), dtype=torch.long, device=device)
+    at = 0
+    for b, n in enumerate(need):
+        table[b, :n] = perm[at:at + n]
+        at += n
+    q = torch.randn(len(contexts), heads, 128, generator=gen, device=device).to(torch.bfloat16)
+    got = data_plane.paged_decode_attention_fp4(q, kp, vp, table, torch.tensor(contexts, device=device), SCALE)
+    got = got.double().view(len(contexts), heads, 128)
+    for b, n in enumerate(contexts):
+        if n == 0:
+            assert not got[b].any()
+            continue
+        k, v = (torch.empty(1, 16 * need[b], kv_heads, 128, dtype=torch.bfloat16, device=device) for _ in range(2))
+        data_plane.gather_blocks_fp4([kp], [vp], table[b:b + 1, :need[b]], [k], [v])
+        for h in range(heads):
+            kh, vh, qh = k[0, :n, h // 2].double(), v[0, :n, h // 2].double(), q[b, h].double()
+            p = torch.softmax(SCALE * (kh * qh).sum(1), 0)
+            ref, weighed = (p[:, None] * vh).sum(0), (p[:, None] * vh.abs()).sum(0)
+            size = SCALE * (kh * qh).abs().sum(1).max()
+            e = torch.expm1(2.0 ** -11 * size)
+            assert ((got[b, h] - ref).abs() <= 2.0 ** -8 * ref.abs() + (2.0 ** -7 + e) * weighed).all(), (b, h)
+
+
 def test_decode_context_beyond_its_table(native_lib, device):
     contexts = [500, 49]
     case = decode_case(4, contexts, 4, 2, width=3)
@@ -109,10 +166,11 @@ def test_decode_larger_blocks(native_lib, device):
     check_decode(run_decode(device, q, kp, vp, blocks, contexts, sub=3), q, kp, vp, table, contexts)
 
 
-def test_decode_hidden_tokens_never_count(native_lib, device):
+@pytest.mark.parametrize("width", [None, 900, 4000])  # whole sequences, parts, streams
+def test_decode_hidden_tokens_never_count(native_lib, device, width):
     """NaN scales after each context, in the null block and in unused blocks change no bit."""
     contexts = [1, 47, 0, 1030, 128]
-    q, kp, vp, table = decode_case(8, contexts, 16, 8)
+    q, kp, vp, table = decode_case(8, contexts, 16, 8, width=width)
     clean = run_decode(device, q, kp, vp, table, contexts)
     for pool, value in ((kp, False), (vp, True)):
         used = np.zeros((pool.shape[0], 16), dtype=bool)
@@ -126,9 +184,10 @@ def test_decode_hidden_tokens_never_count(native_lib, device):
     assert torch.equal(clean.view(torch.int16), dirty.view(torch.int16))
 
 
-def test_decode_visible_nan_reaches_its_output_alone(native_lib, device):
+@pytest.mark.parametrize("width", [None, 21000])  # parts, streams
+def test_decode_visible_nan_reaches_its_output_alone(native_lib, device, width):
     contexts = [40, 41, 1500]
-    q, kp, vp, table = decode_case(9, contexts, 4, 2)
+    q, kp, vp, table = decode_case(9, contexts, 4, 2, width=width)
     kp[table[0, 1], 0, fp4_ref.scale_at(False, 3, 2)] = 255  # sequence 0, KV head 0: every dim
     vp[table[2, 70], 1, fp4_ref.scale_at(True, 5, 1)] = 255  # sequence 2, KV head 1: dims 32 .. 63
     out = run_decode(device, q, kp, vp, table, contexts).view(3, 4, 128).isnan().cpu()
