@@ -175,7 +175,6 @@ __global__ __launch_bounds__(S::kThreads, 2) void fp4_prefill_kernel(const Fp4Pr
   float m_run[kNt];
 #pragma unroll
   for (int nt = 0; nt < kNt; ++nt) m_run[nt] = -INFINITY;
-  f32x4 sacc[4][kNt];
   bf16x8 pf[kNt][2];
   const float scale = a.scale;
 
@@ -186,8 +185,10 @@ __global__ __launch_bounds__(S::kThreads, 2) void fp4_prefill_kernel(const Fp4Pr
 #pragma unroll
   for (int dt = 0; dt < 8; ++dt) v_off[dt] = vr * 256 + (((2 * dt + ((ql >> 1) & 1)) ^ vr) & 15) * 16 + (ql & 1) * 8;
 
-  // Softmax of sacc (raw products): keys key0 .. key0 + 63 at positions of which query i sees [lo, hi(i)].
-  auto tile_softmax = [&](const int key0, const bool hist, const bool need_mask) __attribute__((always_inline)) {
+  // Softmax of raw products x, keys key0 .. key0 + 63, of which query i sees [lo, hi(i)]: first masks and the running
+  // maximum (rarely raised), then the weights.
+  typedef f32x4 scores_t[4][kNt];
+  auto raise_max = [&](scores_t& x, const int key0, const bool hist, const bool need_mask) __attribute__((always_inline)) {
     if (__builtin_expect(__builtin_amdgcn_readfirstlane(static_cast<int>(need_mask)) != 0, 0)) {
 #pragma unroll
       for (int nt = 0; nt < kNt; ++nt) {
@@ -201,7 +202,7 @@ __global__ __launch_bounds__(S::kThreads, 2) void fp4_prefill_kernel(const Fp4Pr
           for (int i = 0; i < 4; ++i) {
             const int kpos = key0 + mt * 16 + 4 * gq + i;
             const bool vis = row_ok & (kpos >= lo) & (kpos <= hi);
-            sacc[mt][nt][i] = vis ? sacc[mt][nt][i] : -INFINITY;
+            x[mt][nt][i] = vis ? x[mt][nt][i] : -INFINITY;
           }
       }
     }
@@ -213,7 +214,7 @@ __global__ __launch_bounds__(S::kThreads, 2) void fp4_prefill_kernel(const Fp4Pr
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v = fmaxf(v, sacc[mt][nt][i]);
+        for (int i = 0; i < 4; ++i) v = fmaxf(v, x[mt][nt][i]);
       mx[nt] = v * scale;
       grow = grow || mx[nt] > m_run[nt] + kRescaleSlack;
     }
@@ -227,21 +228,19 @@ __global__ __launch_bounds__(S::kThreads, 2) void fp4_prefill_kernel(const Fp4Pr
         for (int dt = 0; dt < 9; ++dt) oacc[dt][nt] *= alpha;
       }
     }
+  };
+  auto weights = [&](scores_t& x) __attribute__((always_inline)) {
 #pragma unroll
-    for (int nt = 0; nt < kNt; ++nt) {
-      const float ref = m_run[nt] == -INFINITY ? 0.0f : m_run[nt];
+    for (int ks2 = 0; ks2 < 2; ++ks2)
 #pragma unroll
-      for (int mt = 0; mt < 4; ++mt)
+      for (int nt = 0; nt < kNt; ++nt) {
+        const float ref = m_run[nt] == -INFINITY ? 0.0f : m_run[nt];
+        f32x8 pv;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sacc[mt][nt][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[mt][nt][i], scale, -ref));
-#pragma unroll
-      for (int ks2 = 0; ks2 < 2; ++ks2) {
-        const f32x8 pv = {sacc[2 * ks2][nt][0], sacc[2 * ks2][nt][1], sacc[2 * ks2][nt][2], sacc[2 * ks2][nt][3],
-                          sacc[2 * ks2 + 1][nt][0], sacc[2 * ks2 + 1][nt][1], sacc[2 * ks2 + 1][nt][2],
-                          sacc[2 * ks2 + 1][nt][3]};
+        for (int e = 0; e < 8; ++e)
+          pv[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * ks2 + (e >> 2)][nt][e & 3], scale, -ref));
         pf[nt][ks2] = __builtin_convertvector(pv, bf16x8);
       }
-    }
   };
   auto tile_values = [&](const char* sVb) __attribute__((always_inline)) {
 #pragma unroll
@@ -271,38 +270,61 @@ __global__ __launch_bounds__(S::kThreads, 2) void fp4_prefill_kernel(const Fp4Pr
     const int nhb = (nh + kFp4Tokens - 1) / kFp4Tokens;
     const int64_t block_bytes = static_cast<int64_t>(a.kv_heads) * kFp4Record;
     const int64_t* table = a.history_blocks + b * a.history_stride;
-    // This thread's code words: block my_blk of the tile (the wavefront's), byte my_at of its codes.
-    const int my_blk = __builtin_amdgcn_readfirstlane(gt * kWords * 4 / kFp4Codes);
-    const int my_at = gt * kWords * 4 % kFp4Codes;
-    const int quad = my_at >> 8, octet = (my_at >> 4) & 15, tok = 4 * quad + ((my_at >> 2) & 3);
-    auto block_of = [&](const int t, const int blk) __attribute__((always_inline)) {
-      const int64_t x = table[min(t * kTileBlocks + blk, nhb - 1)];
-      return (x < 0 || x >= a.num_blocks) ? int64_t{0} : x;
+    // This thread's code words of the tile: in block my_blk (the wavefront's), K bytes my_at .. of its codes, and V of octet
+    // gt % 16 and kWords tokens from tok on (16 lanes write a whole LDS row: no bank conflicts).
+    constexpr int kBlockThreads = kFp4Codes / 4 / kWords;  // threads of a block
+    const int my_blk = __builtin_amdgcn_readfirstlane(gt / kBlockThreads);
+    const int my_at = gt % kBlockThreads * 4 * kWords;
+    const int octet = gt & 15, tok = gt % kBlockThreads / 16 * kWords, quad = tok >> 2;
+    const uint32_t v_from = 256 * quad + 16 * octet + 4 * (tok & 3);
+    // Block ids of the tile that is loaded next, fetched a round ahead: this wavefront's block, and block lane / 16 (whose K
+    // scales the lane moves).  Tiles past the last are the last again: their keys are hidden.
+    int64_t id_mine, id_lane;
+    auto fetch_ids = [&](const int t) __attribute__((always_inline)) {
+      id_mine = table[min(t * kTileBlocks + my_blk, nhb - 1)];
+      id_lane = table[min(t * kTileBlocks + gq, nhb - 1)];
+    };
+    const uint32_t blocks_end = static_cast<uint32_t>(a.num_blocks);  // < 2^31, checked by the entry point
+    auto block_of = [&](const int64_t id) __attribute__((always_inline)) {
+      return static_cast<uint64_t>(id) < blocks_end ? static_cast<uint32_t>(id) : 0u;
     };
     typedef uint32_t words_t __attribute__((ext_vector_type(kWords)));
     words_t kw{}, vw{};
     uint32_t vs = 0, ks = 0;
-    auto load = [&](const int t) __attribute__((always_inline)) {
-      const char* k = a.key_pool + block_of(t, my_blk) * block_bytes + g * kFp4Record;
-      const char* v = a.value_pool + block_of(t, my_blk) * block_bytes + g * kFp4Record;
-      kw = *reinterpret_cast<const words_t*>(k + my_at);
-      vw = *reinterpret_cast<const words_t*>(v + my_at);
-      vs = *reinterpret_cast<const uint32_t*>(v + kFp4Codes + 16 * quad + 4 * (octet >> 2));
-      if (wt == 0)  // the tile's K scales: 16 lanes a block
-        ks = *reinterpret_cast<const uint32_t*>(a.key_pool + block_of(t, lane >> 4) * block_bytes + g * kFp4Record +
-                                                kFp4Codes + 4 * ql);
+    const char* const k_base = a.key_pool + g * kFp4Record;
+    const char* const v_base = a.value_pool + g * kFp4Record;
+    const uint32_t vs_at = kFp4Codes + 16 * quad + 4 * (octet >> 2);
+    auto load_tile = [&]() __attribute__((always_inline)) {
+      const int64_t at = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(block_of(id_mine)))) * block_bytes;
+      kw = *reinterpret_cast<const words_t*>(k_base + at + my_at);
+      vw = *reinterpret_cast<const words_t*>(v_base + at + v_from);
+      vs = *reinterpret_cast<const uint32_t*>(v_base + at + vs_at);
+      ks = *reinterpret_cast<const uint32_t*>(k_base + block_of(id_lane) * block_bytes + kFp4Codes + 4 * ql);
     };
-    auto store = [&](const int t, unsigned char* buf) __attribute__((always_inline)) {
+    // Byte offsets of this thread's rows in a V tile, and its shift to the first one's scale.
+    uint32_t v_at[kWords];
+#pragma unroll
+    for (int e = 0; e < kWords; ++e) {
+      const int row = kFp4Tokens * my_blk + tok + e;
+      v_at[e] = row * 256 + ((octet ^ (row & 15)) * 16);
+    }
+    const uint32_t vs_shift = 8 * (tok & 3);
+    auto store_tile = [&](const int t, unsigned char* buf) __attribute__((always_inline)) {
       *reinterpret_cast<words_t*>(buf + kFp4Codes * my_blk + my_at) = kw;
-      if (wt == 0) *reinterpret_cast<uint32_t*>(buf + S::kHistK + 4 * lane) = ks;
-      unsigned char* vt = buf + S::kHistK + S::kHistScales;
-      const bool tail = (t + 1) * kKTile > nh;  // uniform
+      *reinterpret_cast<uint32_t*>(buf + S::kHistK + 4 * lane) = ks;
+      vs >>= vs_shift;
+      if (__builtin_expect((t + 1) * kKTile > nh, 0)) {  // uniform
+#pragma unroll
+        for (int e = 0; e < kWords; ++e)
+          if (t * kKTile + kFp4Tokens * my_blk + tok + e >= nh) {
+            vw[e] = 0;
+            vs &= ~(0xffu << (8 * e));
+          }
+      }
 #pragma unroll
       for (int e = 0; e < kWords; ++e) {
-        const int row = kFp4Tokens * my_blk + tok + e;
-        uint32_t codes = vw[e], s = (vs >> (8 * ((tok + e) & 3))) & 0xffu;
-        if (tail && t * kKTile + row >= nh) codes = s = 0;
-        *reinterpret_cast<u32x4*>(vt + row * 256 + ((octet ^ (row & 15)) * 16)) = fp4_unpack8(codes, e8m0_f32(s));
+        const uint32_t codes = vw[e];
+        *reinterpret_cast<u32x4*>(buf + S::kHistK + S::kHistScales + v_at[e]) = fp4_unpack8(codes, e8m0_f32((vs >> (8 * e)) & 0xffu));
       }
     };
     i32x8 q_hi[kNt], q_lo[kNt];
@@ -319,37 +341,45 @@ __global__ __launch_bounds__(S::kThreads, 2) void fp4_prefill_kernel(const Fp4Pr
       hi_scale[nt] = split.hi;
       lo_scale[nt] = split.lo;
     }
-    if (wk < n_hist) {
-      load(wk);
-      store(wk, lds);
-    }
-    __syncthreads();
-    // Every wavefront passes every barrier: the rounds are uniform, a group without a tile only waits.
-    for (int t0 = 0, buf = 0; t0 < n_hist; t0 += kKeySplit, buf ^= 1) {
-      const int t = t0 + wk;
-      unsigned char* cur = lds + buf * S::kHistBuffer;
-      const bool more = t + kKeySplit < n_hist;
-      if (more) load(t + kKeySplit);
-      if (t < n_hist) {
+    auto products = [&](scores_t& x, const unsigned char* buf) __attribute__((always_inline)) {
 #pragma unroll
-        for (int mt = 0; mt < 4; ++mt) {
-          const u32x4 kc = *reinterpret_cast<const u32x4*>(cur + kFp4Codes * mt + 16 * lane);
-          const int sc = cur[S::kHistK + 64 * mt + lane];
-          i32x8 kf{};
+      for (int mt = 0; mt < 4; ++mt) {
+        const u32x4 kc = *reinterpret_cast<const u32x4*>(buf + kFp4Codes * mt + 16 * lane);
+        const int sc = buf[S::kHistK + 64 * mt + lane];
+        i32x8 kf{};
 #pragma unroll
-          for (int e = 0; e < 4; ++e) kf[e] = kc[e];
+        for (int e = 0; e < 4; ++e) kf[e] = kc[e];
 #pragma unroll
-          for (int nt = 0; nt < kNt; ++nt) {
-            f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-            acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(kf, q_lo[nt], acc, 4, 0, 0, sc, 0, lo_scale[nt]);
-            sacc[mt][nt] =
-                __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(kf, q_hi[nt], acc, 4, 0, 0, sc, 0, hi_scale[nt]);
-          }
+        for (int nt = 0; nt < kNt; ++nt) {
+          f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+          acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(kf, q_lo[nt], acc, 4, 0, 0, sc, 0, lo_scale[nt]);
+          x[mt][nt] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(kf, q_hi[nt], acc, 4, 0, 0, sc, 0, hi_scale[nt]);
         }
-        tile_softmax(t * kKTile, true, (t + 1) * kKTile > nh || rows_edge);
-        tile_values(reinterpret_cast<const char*>(cur + S::kHistK + S::kHistScales));
       }
-      if (more) store(t + kKeySplit, lds + (buf ^ 1) * S::kHistBuffer);
+    };
+    // In round i this group's tile is t = wk + i kKeySplit: it is in LDS, the next one in registers or on its way there, the one
+    // after follows at the round's end.  Every wavefront does every round (the last may be hidden as a whole).
+    // In round i this group's tile is t = wk + i kKeySplit: it is in LDS, the next one goes there in the round, the one after
+    // into registers.  Every wavefront does every round (a group's last may be hidden as a whole).
+    fetch_ids(wk);
+    load_tile();
+    fetch_ids(wk + kKeySplit);
+    store_tile(wk, lds);
+    load_tile();
+    fetch_ids(wk + 2 * kKeySplit);
+    __syncthreads();
+    const int rounds = (n_hist + kKeySplit - 1) / kKeySplit;
+    scores_t sacc;
+    for (int i = 0; i < rounds; ++i) {
+      const int t = wk + i * kKeySplit;
+      unsigned char* const cur = lds + (i & 1) * S::kHistBuffer;
+      products(sacc, cur);
+      store_tile(t + kKeySplit, lds + ((i & 1) ^ 1) * S::kHistBuffer);
+      load_tile();
+      fetch_ids(t + 3 * kKeySplit);
+      raise_max(sacc, t * kKTile, true, (t + 1) * kKTile > nh || rows_edge);
+      weights(sacc);
+      tile_values(reinterpret_cast<const char*>(cur + S::kHistK + S::kHistScales));
       __syncthreads();
     }
   }
@@ -406,6 +436,7 @@ __global__ __launch_bounds__(S::kThreads, 2) void fp4_prefill_kernel(const Fp4Pr
     const char* v_tiles = k_tiles + 2 * kTileBytes;
     auto tile_step = [&](const int t, const int buf) __attribute__((always_inline)) {
       if (t + kKeySplit < n_tiles) dma_tile(t + kKeySplit, buf ^ 1);
+      scores_t sacc;
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt)
 #pragma unroll
@@ -420,7 +451,8 @@ __global__ __launch_bounds__(S::kThreads, 2) void fp4_prefill_kernel(const Fp4Pr
             sacc[mt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[nt][ks], sacc[mt][nt], 0, 0, 0);
         }
       const int key0 = (c_lo + t) * kKTile;
-      tile_softmax(key0, false, key0 + kKTile - 1 > qw0 || key0 < pad || rows_edge);
+      raise_max(sacc, key0, false, key0 + kKTile - 1 > qw0 || key0 < pad || rows_edge);
+      weights(sacc);
       tile_values(v_tiles + buf * kTileBytes);
     };
     // The loads into LDS are the asm's, which the compiler does not count: each wavefront waits for its own before a
