@@ -522,7 +522,9 @@ int32_t mi_copy_blocks(void* const* key_pools, void* const* value_pools, int64_t
  * mi_chunked_prefill_attention_fp4 -- kernel 4 with the history in 4-bit pools and the chunk's own K/V in bf16: the arguments of
  * mi_chunked_prefill_attention (without block_size) and its visibility, scores in fp32.  Padding positions of the
  * chunk and history slots past start_lens never reach an output; the chunk's real K and V rows are taken to be finite
- * (one that is not may also reach queries before it).  max_history_blocks is not limited by LDS.
+ * (one that is not may also reach queries before it).  max_history_blocks is not limited by LDS.  workspace: at least
+ * mi_chunked_prefill_fp4_workspace_bytes(...) bytes, as for decode: short chunks behind a long history have their keys cut over
+ * workgroups, with partials there.
  */
 #define MI_TYPE_BF16 1
 #define MI_TYPE_FP16 2
@@ -556,7 +558,9 @@ int32_t mi_chunked_prefill_attention_fp4(void* out, int64_t out_row_stride, int6
                                          int64_t history_stride, int32_t max_history_blocks, const int64_t* start_lens,
                                          const int64_t* chunk_lens, int64_t lens_stride, int32_t batch,
                                          int32_t padded_len, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
-                                         float scale, void* stream);
+                                         float scale, void* workspace, int64_t workspace_bytes, void* stream);
+int64_t mi_chunked_prefill_fp4_workspace_bytes(int32_t batch, int32_t padded_len, int32_t num_heads,
+                                               int32_t num_kv_heads, int32_t max_history_blocks);
 
 #ifdef __cplusplus
 }

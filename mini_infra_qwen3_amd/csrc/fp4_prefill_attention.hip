@@ -7,16 +7,26 @@
 //
 // One flash-style kernel in two phases that share the softmax state: history tiles, then the chunk's.
 //  * Workgroup: a row, a pair of query heads of one KV head, kQTile queries; wavefronts as (head, queries).  Both
-//    heads share every tile of 64 keys in LDS.
+//    heads share every tile of 64 keys in LDS.  Short chunks behind a long history have the tiles of a row cut into
+//    parts, a workgroup each, and a second launch joins their partials.
 //  * History keys are multiplied as they are stored (v_mfma_scale_f32_16x16x128_f8f6f4): a block's 1 KiB of codes
 //    goes to LDS untouched and is the A operand, 16 bytes a lane, at its 16 scale bytes; B is the query in two 8-bit floats
 //    (split_query).  Two such products take the time of the four bf16 ones, from a quarter of the LDS bytes.
 //  * History values are unpacked to bf16 (exact) on their way to LDS, each once per workgroup, into the layout of the
-//    chunk's: rows of 256 bytes, 16-byte pieces XOR-swizzled by the row.  Tokens past nh become zeros there.
+//    chunk's: rows of 256 bytes, 16-byte pieces XOR-swizzled by the row, sixteen lanes a row (a thread's own eight bytes
+//    in order put two rows' pieces on the same banks).  Tokens past nh become zeros there.
 //  * Chunk tiles go from memory straight into LDS; keys before the row's first token read that token's row.
-//  * P V by v_mfma_f32_16x16x32_bf16: the probabilities are rounded to bf16 (2^-9 of a weight; the output's
-//    own rounding is as large), V^T comes from LDS by transposing reads, and a ninth tile sums the rounded weights.
+//  * P V by v_mfma_f32_16x16x32_bf16: the probabilities are rounded to bf16 (half a step, 2^-8 of a weight, as the
+//    output's own rounding), V^T comes from LDS by transposing reads, and a ninth tile sums the rounded weights.
 //  * Scores stay in fp32; the running maximum is raised only when a score passes it by 2^8.
+//
+// What bounds it (4 x 2048 queries behind 10240 tokens, 600 us, 1260 TFLOP/s; a large bf16 library product reaches 1348
+// on this card): a wavefront's tile is 1088 cycles of matrix unit and about 270 issue slots of 4 cycles of vector work (32
+// exponentials take four slots each), and the two wavefronts of a SIMD do them largely one after the other.  Timing copies
+// of an earlier 635 us: without the softmax 563, without staging 535, without the products with K 517, with V 485.  No gains:
+// a tile's products a round before its softmax (704 to 708 against 683, instructions interleaved by hand or not),
+// LDS reads further ahead by hand (709 to 714 against 622), wave priorities (651 against 635), a barrier every two or
+// three tiles (606, 639 against 601), two workgroups of half the queries a CU (630).
 #include <algorithm>
 #include <initializer_list>
 
@@ -55,6 +65,8 @@ using Wide = Shape<2, 4, 1>;       // 128 queries, 8 wavefronts
 using Half = Shape<2, 2, 1>;       // 64 queries, 4 wavefronts
 using HalfSplit = Shape<2, 2, 2>;  // 64 queries, 8 wavefronts, the keys in two halves
 using Narrow = Shape<1, 2, 2>;     // 32 queries, 8 wavefronts, the keys in two halves
+using Slim = Shape<1, 2, 1>;       // 32 queries, 4 wavefronts; the form for keys cut over workgroups
+constexpr int kMergeThreads = 256;
 
 struct Fp4PrefillArgs {
   uint16_t* out;
@@ -82,6 +94,9 @@ struct Fp4PrefillArgs {
   uint32_t q_sign;
   int32_t tiles;  // query tiles per row
   int32_t batch;
+  int32_t parts;  // workgroups that share the keys of a query tile, each writing partials (1: the output)
+  float* ws_acc;  // [batch, heads, padded_len, parts, 128]
+  float* ws_ml;   // [batch, heads, padded_len, parts, 2]: max (log2 units) and sum
   int32_t round_pairs;  // (row, head pair) units per dispatch round of one workgroup queue
 };
 
@@ -102,11 +117,12 @@ __global__ __launch_bounds__(S::kThreads, 2) void fp4_prefill_kernel(const Fp4Pr
 
   // Workgroup -> (row b, head pair hp, query tile qt): the tiles of a pair on one XCD, heaviest first within rounds
   // of as many pairs as the XCD's CUs hold (as mi_chunked_prefill_attention).
-  int b, hp, qt;
+  int b, hp, qt, part;
   {
     const int tiles = a.tiles;
     const int per_row = a.kv_heads * a.pairs;
-    const int pairs = per_row * a.batch;
+    const int rows_pairs = per_row * a.batch;
+    const int pairs = rows_pairs * a.parts;
     const int lin = static_cast<int>(blockIdx.x);
     const bool by_xcd = pairs % kXcds == 0;
     const int units = by_xcd ? pairs / kXcds : pairs;
@@ -118,8 +134,9 @@ __global__ __launch_bounds__(S::kThreads, 2) void fp4_prefill_kernel(const Fp4Pr
     const int unit = round_idx * a.round_pairs + (within - rank * round_size);
     const int pair = by_xcd ? unit * kXcds + lin % kXcds : unit;
     // (divisions run on the vector unit: back to scalars, which the addresses need)
+    part = __builtin_amdgcn_readfirstlane(pair / rows_pairs);
     hp = __builtin_amdgcn_readfirstlane(pair % per_row);
-    b = __builtin_amdgcn_readfirstlane(pair / per_row);
+    b = __builtin_amdgcn_readfirstlane(pair % rows_pairs / per_row);
     qt = __builtin_amdgcn_readfirstlane(tiles - 1 - rank);
   }
   const int q0 = qt * kQTile;
@@ -149,6 +166,7 @@ __global__ __launch_bounds__(S::kThreads, 2) void fp4_prefill_kernel(const Fp4Pr
 
   uint16_t* out_b = a.out + b * a.out_row;
   if (q0 + kQTile <= pad) {  // the whole tile is padding: zero rows
+    if (a.parts > 1) return;  // the second launch's
     for (int c = tid; c < kQTile * kGroup * (kHeadDim / 8); c += kThreads) {
       const int qi = q0 + c / (kGroup * (kHeadDim / 8));
       const int rem = c % (kGroup * (kHeadDim / 8));
@@ -185,17 +203,16 @@ __global__ __launch_bounds__(S::kThreads, 2) void fp4_prefill_kernel(const Fp4Pr
 #pragma unroll
   for (int dt = 0; dt < 8; ++dt) v_off[dt] = vr * 256 + (((2 * dt + ((ql >> 1) & 1)) ^ vr) & 15) * 16 + (ql & 1) * 8;
 
-  // Softmax of raw products x, keys key0 .. key0 + 63, of which query i sees [lo, hi(i)]: first masks and the running
-  // maximum (rarely raised), then the weights.
+  // Softmax of raw products x, keys key0 .. key0 + 63, of which query i sees [lo, last] (last < 0: [lo, i]): first masks
+  // and the running maximum (rarely raised), then the weights.
   typedef f32x4 scores_t[4][kNt];
-  auto raise_max = [&](scores_t& x, const int key0, const bool hist, const bool need_mask) __attribute__((always_inline)) {
+  auto raise_max = [&](scores_t& x, const int key0, const int lo, const int last, const bool need_mask) __attribute__((always_inline)) {
     if (__builtin_expect(__builtin_amdgcn_readfirstlane(static_cast<int>(need_mask)) != 0, 0)) {
 #pragma unroll
       for (int nt = 0; nt < kNt; ++nt) {
         const int qi = qw0 + 16 * nt + ql;
         const bool row_ok = (qi >= pad) & (qi < L);
-        const int lo = hist ? 0 : pad;
-        const int hi = hist ? nh - 1 : qi;
+        const int hi = last < 0 ? qi : last;
 #pragma unroll
         for (int mt = 0; mt < 4; ++mt)
 #pragma unroll
@@ -264,9 +281,18 @@ __global__ __launch_bounds__(S::kThreads, 2) void fp4_prefill_kernel(const Fp4Pr
   unsigned char* lds = s_raw + wk * S::kGroupLds;
   const bool rows_edge = qw0 < pad || qw0 + kQPerWave - 1 >= L;  // some of the wavefront's queries are none
 
+  // This workgroup's tiles of the row's: history tiles [h0, h1), then chunk tiles [c0, c1) (all, unless parts share them).
+  const int hist_tiles = (nh + kKTile - 1) / kKTile;
+  const int c_first = pad / kKTile;
+  const int all_tiles = hist_tiles + (min(q0 + kQTile, L) - 1) / kKTile - c_first + 1;
+  const int t_begin = static_cast<int>(static_cast<int64_t>(all_tiles) * part / a.parts);
+  const int t_end = static_cast<int>(static_cast<int64_t>(all_tiles) * (part + 1) / a.parts);
+  const int h0 = min(t_begin, hist_tiles), h1 = min(t_end, hist_tiles);
+  const int c0 = c_first + max(t_begin - hist_tiles, 0), c1 = c_first + max(t_end - hist_tiles, 0);
+
   // ---- Phase 1: the history.  Per buffer: 4 KiB of K codes, 256 K scale bytes, the bf16 V tile.
-  const int n_hist = (nh + kKTile - 1) / kKTile;
-  if (n_hist > 0) {  // uniform
+  if (h1 > h0) {  // uniform
+    const int seen = min(nh, h1 * kKTile);  // history keys that this workgroup shows its queries
     const int nhb = (nh + kFp4Tokens - 1) / kFp4Tokens;
     const int64_t block_bytes = static_cast<int64_t>(a.kv_heads) * kFp4Record;
     const int64_t* table = a.history_blocks + b * a.history_stride;
@@ -313,10 +339,10 @@ __global__ __launch_bounds__(S::kThreads, 2) void fp4_prefill_kernel(const Fp4Pr
       *reinterpret_cast<words_t*>(buf + kFp4Codes * my_blk + my_at) = kw;
       *reinterpret_cast<uint32_t*>(buf + S::kHistK + 4 * lane) = ks;
       vs >>= vs_shift;
-      if (__builtin_expect((t + 1) * kKTile > nh, 0)) {  // uniform
+      if (__builtin_expect((t + 1) * kKTile > seen, 0)) {  // uniform
 #pragma unroll
         for (int e = 0; e < kWords; ++e)
-          if (t * kKTile + kFp4Tokens * my_blk + tok + e >= nh) {
+          if (t * kKTile + kFp4Tokens * my_blk + tok + e >= seen) {
             vw[e] = 0;
             vs &= ~(0xffu << (8 * e));
           }
@@ -357,27 +383,25 @@ __global__ __launch_bounds__(S::kThreads, 2) void fp4_prefill_kernel(const Fp4Pr
         }
       }
     };
-    // In round i this group's tile is t = wk + i kKeySplit: it is in LDS, the next one in registers or on its way there, the one
-    // after follows at the round's end.  Every wavefront does every round (the last may be hidden as a whole).
-    // In round i this group's tile is t = wk + i kKeySplit: it is in LDS, the next one goes there in the round, the one after
+    // In round i this group's tile is t = h0 + wk + i kKeySplit: it is in LDS, the next one goes there in the round, the one after
     // into registers.  Every wavefront does every round (a group's last may be hidden as a whole).
-    fetch_ids(wk);
+    fetch_ids(h0 + wk);
     load_tile();
-    fetch_ids(wk + kKeySplit);
-    store_tile(wk, lds);
+    fetch_ids(h0 + wk + kKeySplit);
+    store_tile(h0 + wk, lds);
     load_tile();
-    fetch_ids(wk + 2 * kKeySplit);
+    fetch_ids(h0 + wk + 2 * kKeySplit);
     __syncthreads();
-    const int rounds = (n_hist + kKeySplit - 1) / kKeySplit;
+    const int rounds = (h1 - h0 + kKeySplit - 1) / kKeySplit;
     scores_t sacc;
     for (int i = 0; i < rounds; ++i) {
-      const int t = wk + i * kKeySplit;
+      const int t = h0 + wk + i * kKeySplit;
       unsigned char* const cur = lds + (i & 1) * S::kHistBuffer;
       products(sacc, cur);
       store_tile(t + kKeySplit, lds + ((i & 1) ^ 1) * S::kHistBuffer);
       load_tile();
       fetch_ids(t + 3 * kKeySplit);
-      raise_max(sacc, t * kKTile, true, (t + 1) * kKTile > nh || rows_edge);
+      raise_max(sacc, t * kKTile, 0, seen - 1, (t + 1) * kKTile > seen || rows_edge);
       weights(sacc);
       tile_values(reinterpret_cast<const char*>(cur + S::kHistK + S::kHistScales));
       __syncthreads();
@@ -386,9 +410,8 @@ __global__ __launch_bounds__(S::kThreads, 2) void fp4_prefill_kernel(const Fp4Pr
 
   // ---- Phase 2: the chunk, bf16 tiles in double-buffered LDS (two K tiles, then two V tiles).
   {
-    const int c_lo = pad / kKTile;
-    const int c_hi = (min(q0 + kQTile, L) - 1) / kKTile;
-    const int n_tiles = c_hi - c_lo + 1;
+    const int c_lo = c0;
+    const int n_tiles = c1 - c0;
     bf16x8 qf[kNt][4];
 #pragma unroll
     for (int nt = 0; nt < kNt; ++nt) {
@@ -451,7 +474,7 @@ __global__ __launch_bounds__(S::kThreads, 2) void fp4_prefill_kernel(const Fp4Pr
             sacc[mt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[nt][ks], sacc[mt][nt], 0, 0, 0);
         }
       const int key0 = (c_lo + t) * kKTile;
-      raise_max(sacc, key0, false, key0 + kKTile - 1 > qw0 || key0 < pad || rows_edge);
+      raise_max(sacc, key0, pad, -1, key0 + kKTile - 1 > qw0 || key0 < pad || rows_edge);
       weights(sacc);
       tile_values(v_tiles + buf * kTileBytes);
     };
@@ -507,6 +530,19 @@ __global__ __launch_bounds__(S::kThreads, 2) void fp4_prefill_kernel(const Fp4Pr
       }
     }
   }
+  if (a.parts > 1) {  // unnormalised sums; padding rows are the second launch's
+#pragma unroll
+    for (int nt = 0; nt < kNt; ++nt) {
+      const int qi = qw0 + 16 * nt + ql;
+      if (qi >= L || qi < pad || !head_live) continue;
+      const int64_t slot = ((static_cast<int64_t>(b) * a.kv_heads * a.group + h) * L + qi) * a.parts + part;
+      float* acc = a.ws_acc + slot * kHeadDim + 4 * gq;
+#pragma unroll
+      for (int dt = 0; dt < 8; ++dt) *reinterpret_cast<f32x4*>(acc + 16 * dt) = oacc[dt][nt];
+      if (gq == 0) *reinterpret_cast<float2*>(a.ws_ml + 2 * slot) = make_float2(m_run[nt], oacc[8][nt][0]);
+    }
+    return;
+  }
   // ---- normalise and write: lane holds query qw0 + 16 nt + ql, dims 16 dt + 4 gq + i; padding rows are zeros
 #pragma unroll
   for (int nt = 0; nt < kNt; ++nt) {
@@ -525,10 +561,39 @@ __global__ __launch_bounds__(S::kThreads, 2) void fp4_prefill_kernel(const Fp4Pr
   }
 }
 
+// Joins the parts of every query: 32 threads, four dims each, for a query of a head.
+__global__ __launch_bounds__(kMergeThreads) void fp4_prefill_merge_kernel(const Fp4PrefillArgs a) {
+  const int64_t heads = static_cast<int64_t>(a.kv_heads) * a.group;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * (kMergeThreads / 32) + threadIdx.x / 32;  // (b, query, head)
+  if (row >= heads * a.padded_len * a.batch) return;
+  const int64_t h = row % heads, qi = row / heads % a.padded_len, b = row / heads / a.padded_len;
+  const int x = threadIdx.x & 31;
+  uint16_t* out = a.out + b * a.out_row + qi * a.out_tok + h * kHeadDim + 4 * x;
+  const int64_t len = a.chunk_lens[b * a.lens_stride];
+  if (qi < a.padded_len - len) {
+    *reinterpret_cast<uint2*>(out) = uint2{0u, 0u};
+    return;
+  }
+  const int64_t at = ((b * heads + h) * a.padded_len + qi) * a.parts;
+  float M = -INFINITY;
+  for (int p = 0; p < a.parts; ++p) M = fmaxf(M, a.ws_ml[2 * (at + p)]);
+  float L = 0.0f;
+  f32x4 o{};
+  for (int p = 0; p < a.parts; ++p) {
+    const float2 ml = *reinterpret_cast<const float2*>(a.ws_ml + 2 * (at + p));
+    // A part without a visible key has no sums, except where every score was NaN: then its sum is.
+    const float e = ml.x == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(ml.x - M);
+    L += e * ml.y;
+    o += e * *reinterpret_cast<const f32x4*>(a.ws_acc + (at + p) * kHeadDim + 4 * x);
+  }
+  const float inv = 1.0f / L;
+  *reinterpret_cast<uint2*>(out) = uint2{pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv)};
+}
+
 template <typename S>
 int32_t launch(const char* name, Fp4PrefillArgs& a, hipStream_t s) {
   a.tiles = (a.padded_len + S::kQTile - 1) / S::kQTile;
-  const int64_t pairs = static_cast<int64_t>(a.kv_heads) * a.pairs * a.batch;
+  const int64_t pairs = static_cast<int64_t>(a.kv_heads) * a.pairs * a.batch * a.parts;
   const int64_t groups = a.tiles * pairs;
   if (groups > 0xffffffffll / S::kThreads || groups > 0x3fffffff)
     return fail(MI_ERR_UNSUPPORTED, "%s: too many workgroups", name);
@@ -538,28 +603,90 @@ int32_t launch(const char* name, Fp4PrefillArgs& a, hipStream_t s) {
   a.round_pairs = static_cast<int32_t>(std::max(std::min(cus / a.tiles, units), int64_t{1}));
   if (const int32_t rc = allow_lds<&fp4_prefill_kernel<S>>(S::kLdsBytes, name)) return rc;
   fp4_prefill_kernel<S><<<static_cast<uint32_t>(groups), S::kThreads, S::kLdsBytes, s>>>(a);
+  if (const int32_t rc = check_launch(name)) return rc;
+  if (a.parts == 1) return ok();
+  const int64_t rows = static_cast<int64_t>(a.kv_heads) * a.group * a.padded_len * a.batch;
+  const int64_t merges = (rows * 32 + kMergeThreads - 1) / kMergeThreads;
+  fp4_prefill_merge_kernel<<<static_cast<uint32_t>(merges), kMergeThreads, 0, s>>>(a);
   return check_launch(name);
 }
 
-enum class Form { kWide, kHalf, kHalfSplit, kNarrow };
+enum class Form { kWide, kHalf, kHalfSplit, kNarrow, kSlim };
 
-// The workgroup shape of a launch, by the workgroups it would have in the narrow and the wide shape.
-Form form_for(const Fp4PrefillArgs& a) {
-  const int64_t cus = device_cus();
-  const int64_t pairs = static_cast<int64_t>(a.kv_heads) * a.pairs * a.batch;
-  const int64_t wide = pairs * ((a.padded_len + Wide::kQTile - 1) / Wide::kQTile);
-  const int64_t narrow = pairs * ((a.padded_len + Narrow::kQTile - 1) / Narrow::kQTile);
-  const int64_t history = static_cast<int64_t>(a.max_history_blocks) * kFp4Tokens;
-  if (8 * narrow <= (2 * history >= a.padded_len ? 8 : 11) * cus) return Form::kNarrow;
-  if (history == 0 && a.padded_len <= 256) return Form::kHalf;
-  if (2 * wide <= cus) return Form::kHalfSplit;
-  if (wide <= cus && history >= a.padded_len) return Form::kWide;
-  if (wide <= cus) return a.padded_len > 640 ? Form::kHalfSplit : Form::kHalf;
-  return 16 * wide <= 25 * cus ? Form::kHalf : Form::kWide;
-}
+// The workgroup shape of a launch, by the workgroups it would have in the narrow and the wide shape, and the parts of its keys.
+// Measured, us (16 query, 8 KV heads; rows x queries behind tokens of history, and the workgroups that decide),
+// wide / half / half split / narrow, and the keys cut into 4 / 8 / 16 parts:
+//   parts: twice the CUs' narrow workgroups, six tiles a part at least, three parts at least
+//     1 x 1 behind 4000        8 narrow      138 / 105 /  76 /  53      27 / 20 / 18
+//     1 x 16 behind 20000      8             645 / 490 / 331 / 215      96 / 55 / 37
+//     1 x 60 behind 4000      16             140 / 110 /  79 /  52      29 / 24 / 23
+//     4 x 60 behind 2000      64              78 /  61 /  47 /  31      26 / 27 / 37
+//     1 x 300 behind 4000     80             148 / 116 /  84 /  57      40 / 42 / 49
+//     1 x 512 behind 8000    128             219 / 153 / 123 /  88      63 / 68 / 81
+//   narrow: one round of its workgroups (cus; 11/8 of that without much history)
+//     2 x 333 behind 1500    176 narrow       68 /  53 /  41 /  29      35 / 39 / 56
+//     1 x 1000               256              41 /  34 /  26 /  19
+//   half: short rows without history
+//     15 x 128               120 wide         14 /  10 /  12 /  14
+//     64 x 128               512              34 /  29 /  44 /  52
+//     40 x 256               640              50 /  39 /  57 /  71
+//   half split: up to half of cus wide workgroups, up to 17/16 of them for rows of more than 256; then half for shorter ones
+//     3 x 450                 96              24 /  19 /  16 /  18
+//     16 x 128 behind 1000   128              46 /  34 /  32 /  40
+//     1 x 2000 behind 2000   128             142 / 114 /  81 /  81
+//     20 x 128 behind 2000   160              72 /  64 /  72 /  78
+//     3 x 700                144              30 /  27 /  23 /  25
+//     2 x 1800 behind 4000   240             198 / 170 / 137 / 184
+//     1 x 4096               256             105 /  94 /  82 / 108
+//     3 x 1408 behind 6000   264             322 / 244 / 233 / 301
+//   half: a second wide round at most 9/16 full
+//     3 x 2048               384              77 /  76 /  86 /  99
+//     25 x 256 behind 2000   400             135 / 125 / 153 / 188
+//   wide beyond
+//     4 x 1600               416              63 /  68 /  71 /  92
+//     4 x 1900 behind 1000   480             122 / 143 / 144 / 194
+//     4 x 2048 behind 10240  512             600 / 630 / 639 / 878
+struct Plan {
+  Form form;
+  int32_t parts = 1;
+  int64_t slots = 0;  // partials
+  Plan(int32_t batch, int32_t padded_len, int32_t num_heads, int32_t num_kv_heads, int32_t max_history_blocks) {
+    const int64_t cus = device_cus();
+    const int64_t pairs = static_cast<int64_t>(num_kv_heads) * ((num_heads / num_kv_heads + kGroup - 1) / kGroup) * batch;
+    const int64_t wide = pairs * ((padded_len + Wide::kQTile - 1) / Wide::kQTile);
+    const int64_t narrow = pairs * ((padded_len + Narrow::kQTile - 1) / Narrow::kQTile);
+    const int64_t history = static_cast<int64_t>(max_history_blocks) * kFp4Tokens;
+    const int64_t most = std::min(2 * cus / narrow, (history + padded_len) / (6 * kKTile));
+    if (most >= 3) {
+      form = Form::kSlim;
+      parts = static_cast<int32_t>(most);
+      slots = static_cast<int64_t>(batch) * num_heads * padded_len * parts;
+    } else if (8 * narrow <= (2 * history >= padded_len ? 8 : 11) * cus) {
+      form = Form::kNarrow;
+    } else if (history == 0 && padded_len <= 256) {
+      form = Form::kHalf;
+    } else if (2 * wide <= cus) {
+      form = Form::kHalfSplit;
+    } else if (16 * wide <= 17 * cus) {
+      form = padded_len > 256 ? Form::kHalfSplit : Form::kHalf;
+    } else {
+      form = 16 * wide <= 25 * cus ? Form::kHalf : Form::kWide;
+    }
+  }
+  int64_t bytes() const { return slots * (kHeadDim + 2) * static_cast<int64_t>(sizeof(float)); }
+};
 
 }  // namespace
 }  // namespace mi
+
+extern "C" int64_t mi_chunked_prefill_fp4_workspace_bytes(int32_t batch, int32_t padded_len, int32_t num_heads,
+                                                          int32_t num_kv_heads, int32_t max_history_blocks) {
+  using namespace mi;
+  if (batch <= 0 || padded_len <= 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0 ||
+      max_history_blocks < 0)
+    return 0;
+  return Plan(batch, padded_len, num_heads, num_kv_heads, max_history_blocks).bytes();
+}
 
 extern "C" int32_t mi_chunked_prefill_attention_fp4(
     void* out, int64_t out_row_stride, int64_t out_tok_stride, const void* query, int64_t query_row_stride,
@@ -568,7 +695,8 @@ extern "C" int32_t mi_chunked_prefill_attention_fp4(
     int64_t value_head_stride, int64_t value_tok_stride, const void* key_pool, const void* value_pool,
     int64_t num_blocks, const int64_t* history_blocks, int64_t history_stride, int32_t max_history_blocks,
     const int64_t* start_lens, const int64_t* chunk_lens, int64_t lens_stride, int32_t batch, int32_t padded_len,
-    int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, float scale, void* stream) {
+    int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, float scale, void* workspace, int64_t workspace_bytes,
+    void* stream) {
   using namespace mi;
   const char* name = "mi_chunked_prefill_attention_fp4";
   if (batch < 0 || padded_len < 0 || max_history_blocks < 0 || num_blocks < 0)
@@ -634,11 +762,22 @@ extern "C" int32_t mi_chunked_prefill_attention_fp4(
   a.batch = batch;
   if (static_cast<int64_t>(num_kv_heads) * a.pairs * batch > 0x3fffffff)
     return fail(MI_ERR_UNSUPPORTED, "%s: too many workgroups", name);
+  const Plan plan(batch, padded_len, num_heads, num_kv_heads, max_history_blocks);
+  if (plan.slots > 0) {
+    if (!workspace || workspace_bytes < plan.bytes())
+      return fail(MI_ERR_WORKSPACE, "%s: workspace of %lld bytes needed, got %lld", name, static_cast<long long>(plan.bytes()),
+                  static_cast<long long>(workspace_bytes));
+    if (!aligned16(workspace)) return fail(MI_ERR_UNSUPPORTED, "%s: workspace must be 16-byte aligned", name);
+    a.ws_acc = static_cast<float*>(workspace);
+    a.ws_ml = a.ws_acc + plan.slots * kHeadDim;
+  }
+  a.parts = plan.parts;
   hipStream_t s = as_stream(stream);
-  switch (form_for(a)) {
+  switch (plan.form) {
     case Form::kWide: return launch<Wide>(name, a, s);
     case Form::kHalf: return launch<Half>(name, a, s);
     case Form::kHalfSplit: return launch<HalfSplit>(name, a, s);
-    default: return launch<Narrow>(name, a, s);
+    case Form::kNarrow: return launch<Narrow>(name, a, s);
+    default: return launch<Slim>(name, a, s);
   }
 }

@@ -20,6 +20,7 @@ __all__ = [
     "argmax_rows",
     "chunked_prefill_attention",
     "chunked_prefill_attention_fp4",
+    "chunked_prefill_fp4_workspace_bytes",
     "copy_blocks",
     "fp4_pool_shape",
     "gather_blocks",
@@ -1113,6 +1114,18 @@ def gather_blocks_fp4(
           num_layers, num_kv_heads, 128, _stream(device))
 
 
+def _workspace(workspace: torch.Tensor | None, need: int, device: torch.device) -> tuple[int | None, int, torch.Tensor | None]:
+    """(pointer, bytes, buffer) of a workspace of at least ``need`` bytes: ``workspace`` when it is large enough, else a new
+    buffer, which the caller keeps until the launch is enqueued; (None, 0, None) when nothing is needed."""
+    if need <= 0:
+        return None, 0, None
+    if workspace is None or workspace.numel() * workspace.element_size() < need:
+        workspace = torch.empty(need, dtype=torch.uint8, device=device)
+    elif workspace.device != device or not workspace.is_contiguous():
+        raise ValueError(f"workspace must be contiguous on {device}")
+    return workspace.data_ptr(), workspace.numel() * workspace.element_size(), workspace
+
+
 def paged_decode_fp4_workspace_bytes(batch: int, max_blocks: int, num_heads: int, num_kv_heads: int,
                                      block_size: int = KERNEL_BLOCK_SIZE) -> int:
     """Workspace for ``paged_decode_attention_fp4`` on ``[batch, max_blocks]`` tables (0: none needed)."""
@@ -1167,13 +1180,7 @@ def paged_decode_attention_fp4(
     if batch > 1 and context_lens.stride(0) <= 0:
         context_lens = context_lens.contiguous()
     need = _native.load().mi_paged_decode_fp4_workspace_bytes(batch, max_blocks, num_heads, num_kv_heads)
-    ws_ptr, ws_bytes = None, 0
-    if need > 0:
-        if workspace is None or workspace.numel() * workspace.element_size() < need:
-            workspace = torch.empty(need, dtype=torch.uint8, device=device)
-        elif workspace.get_device() != index or not workspace.is_contiguous():
-            raise ValueError(f"workspace must be contiguous on {device}")
-        ws_ptr, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    ws_ptr, ws_bytes, workspace = _workspace(workspace, need, device)
     _call(device, "mi_paged_decode_attention_fp4", out.data_ptr(), out.stride(0) if batch > 1 else num_heads * head_dim,
           query.data_ptr(), query.stride(0) if batch > 1 else num_heads * head_dim,
           query.stride(1) if num_heads > 1 else head_dim, key_pool.data_ptr(), value_pool.data_ptr(), num_blocks,
@@ -1181,6 +1188,13 @@ def paged_decode_attention_fp4(
           context_lens.data_ptr(), context_lens.stride(0) if batch > 1 else 1, batch, num_heads, num_kv_heads, head_dim,
           float(scale), ws_ptr, ws_bytes, _stream(device))
     return out
+
+
+def chunked_prefill_fp4_workspace_bytes(batch: int, padded_len: int, num_heads: int, num_kv_heads: int, history_blocks: int,
+                                        block_size: int = KERNEL_BLOCK_SIZE) -> int:
+    """Workspace for ``chunked_prefill_attention_fp4`` with tables of ``history_blocks`` (0: none needed)."""
+    return int(_native.load().mi_chunked_prefill_fp4_workspace_bytes(
+        batch, padded_len, num_heads, num_kv_heads, history_blocks * max(block_size // KERNEL_BLOCK_SIZE, 1)))
 
 
 def chunked_prefill_attention_fp4(
@@ -1194,12 +1208,15 @@ def chunked_prefill_attention_fp4(
     chunk_lens: torch.Tensor,
     scale: float,
     out: torch.Tensor | None = None,
+    workspace: torch.Tensor | None = None,
 ) -> torch.Tensor:
     """``chunked_prefill_attention`` with the history read from 4-bit pools (``fp4_pool_shape``).
 
     query ``[B, H, L, 128]``; key / value ``[B, H_kv, L, 128]`` bf16 (left-padded chunk, D contiguous, any other
     strides); history_blocks ``[B, nb]`` int64 (may have ``nb = 0``); start_lens / chunk_lens ``[B]`` int64.
-    Returns ``out`` ``[B, L, H * 128]`` bf16; left-padding rows are zero.
+    Returns ``out`` ``[B, L, H * 128]`` bf16; left-padding rows are zero.  ``workspace`` (optional, uint8, reused
+    across calls of one stream) holds the partials of short chunks behind long histories; it is allocated here when
+    missing or too small.
     """
     pool0 = _require_fp4_pools((key_pool,), (value_pool,))
     device, index = pool0.device, pool0.get_device()
@@ -1235,6 +1252,9 @@ def chunked_prefill_attention_fp4(
         history_blocks = history_blocks.contiguous()
     if batch > 1 and (start_lens.stride(0) != chunk_lens.stride(0) or start_lens.stride(0) <= 0):
         start_lens, chunk_lens = start_lens.contiguous(), chunk_lens.contiguous()
+    need = _native.load().mi_chunked_prefill_fp4_workspace_bytes(batch, padded_len, num_heads, num_kv_heads, nb)
+    ws_ptr, ws_bytes, workspace = _workspace(workspace, need, device)
+
     def strides(t):  # of a dim of one element any stride is good
         return [st if n > 1 else 0 for st, n in zip(t.stride()[:-1], t.shape)]
 
@@ -1243,5 +1263,5 @@ def chunked_prefill_attention_fp4(
           key_pool.data_ptr(), value_pool.data_ptr(), num_blocks, history_blocks.data_ptr() if nb else None,
           (history_blocks.stride(0) if batch > 1 else nb) if nb else 0, nb, start_lens.data_ptr(), chunk_lens.data_ptr(),
           start_lens.stride(0) if batch > 1 else 1, batch, padded_len, num_heads, num_kv_heads, head_dim, float(scale),
-          _stream(device))
+          ws_ptr, ws_bytes, _stream(device))
     return out

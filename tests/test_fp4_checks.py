@@ -86,14 +86,16 @@ def test_decode_workspace_sizes(native_lib):
     ({"batch": -1}, BAD), ({"batch": 0}, OK), ({"L": 0}, OK), ({"q": None}, BAD), ({"hist": None}, BAD), ({"blocks": 0}, BAD),
     ({"dim": 64}, UNSUPPORTED), ({"heads": 20}, UNSUPPORTED), ({"q_tok": 2052}, UNSUPPORTED), ({"k": 8}, UNSUPPORTED),
     ({"stride": 3}, BAD), ({"lens_stride": 0}, BAD), ({"k_tok": 1 << 24}, UNSUPPORTED), ({"pool": 8}, UNSUPPORTED),
-    ({"nb": 1 << 27, "stride": 1 << 27}, UNSUPPORTED), ({"scale": float("inf")}, BAD), ({"batch": 1 << 28}, UNSUPPORTED)])
+    ({"nb": 1 << 27, "stride": 1 << 27}, UNSUPPORTED), ({"scale": float("inf")}, BAD), ({"batch": 1 << 28}, UNSUPPORTED),
+    ({"nb": 4000, "stride": 4000, "ws": None}, WORKSPACE), ({"nb": 4000, "stride": 4000, "ws_bytes": 64}, WORKSPACE),
+    ({"nb": 4000, "stride": 4000, "ws": 24}, UNSUPPORTED)])
 def test_prefill_refusals(native_lib, change, code):
     a = {"batch": 2, "L": 32, "q": 16, "hist": 16, "blocks": 64, "dim": 128, "heads": 16, "q_tok": 2048, "k": 16, "stride": 4,
-         "lens_stride": 1, "k_tok": 1024, "pool": 16, "nb": 4, "scale": 0.1, **change}
+         "lens_stride": 1, "k_tok": 1024, "pool": 16, "nb": 4, "scale": 0.1, "ws": 16, "ws_bytes": 1 << 40, **change}
     assert native_lib.mi_chunked_prefill_attention_fp4(
         16, 65536, 2048, a["q"], 65536, 128, a["q_tok"], a["k"], 32768, 128, a["k_tok"], 16, 32768, 128, 1024, a["pool"], 16,
         a["blocks"], a["hist"], a["stride"], a["nb"], 16, 16, a["lens_stride"], a["batch"], a["L"], a["heads"], 8, a["dim"],
-        a["scale"], None) == code
+        a["scale"], a["ws"], a["ws_bytes"], None) == code
 
 
 @host_only

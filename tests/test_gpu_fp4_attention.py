@@ -319,6 +319,7 @@ def test_prefill_lengths(native_lib, device, starts, lens, width):
     (3, 450, 70, 16, 8),
     (8, 700, 90, 16, 8),
     (20, 130, 0, 16, 8),
+    (20, 130, 60, 16, 8),
     (6, 1500, 33, 16, 8)])    # many: wide tiles
 def test_prefill_workgroup_shapes(native_lib, device, rows, width, past, heads, kv_heads):
     starts = [max(past - 5 * b, 0) for b in range(rows)]
@@ -326,6 +327,28 @@ def test_prefill_workgroup_shapes(native_lib, device, rows, width, past, heads, 
     case = prefill_case(rows, starts, lens, width, heads, kv_heads)
     queries = sorted({0, 31, 32, 63, 64, 127, 128, width // 2, width - 65, width - 64, width - 2, width - 1})
     check_prefill(run_prefill(device, case, starts, lens), case, starts, lens, queries=queries)
+
+
+@pytest.mark.parametrize("starts,lens,width,table,heads,kv_heads", [
+    ([0], [1], 1, 300, 4, 2),                      # many parts, next to nothing in them
+    ([4700], [1], 1, 300, 4, 2),
+    ([3000, 0, 17, 2999], [40, 33, 0, 1], 40, 200, 16, 8),
+    ([1100, 1023], [70, 12], 70, 80, 5, 1),
+    ([64 * 18], [64], 64, 72, 4, 4),               # parts that end on the chunk's first tile
+    ([900], [200], 200, 60, 2, 1)])
+def test_prefill_parts(native_lib, device, starts, lens, width, table, heads, kv_heads):
+    """Short chunks with wide history tables: the keys of a row cut over workgroups."""
+    assert data_plane.chunked_prefill_fp4_workspace_bytes(len(starts), width, heads, kv_heads, table) > 0
+    case = prefill_case(width + table, starts, lens, width, heads, kv_heads)
+    wide = np.zeros((len(starts), table), dtype=np.int64)
+    wide[:, :case[5].shape[1]] = case[5]
+    case = (*case[:5], wide)
+    out = run_prefill(device, case, starts, lens)
+    check_prefill(out, case, starts, lens)
+    need = data_plane.chunked_prefill_fp4_workspace_bytes(len(starts), width, heads, kv_heads, table)
+    workspace = torch.full((need + 64,), 255, dtype=torch.uint8, device=device)  # NaN: what is read was written
+    again = run_prefill(device, case, starts, lens, workspace=workspace)
+    assert torch.equal(out, again) and (workspace[need:] == 255).all()
 
 
 @pytest.mark.parametrize("scale", [-0.11, 0.0, 1.3])
@@ -357,12 +380,13 @@ def test_prefill_larger_blocks(native_lib, device):
     check_prefill(got, (q, k, v, kp, vp, table), starts, lens)
 
 
-@pytest.mark.parametrize("rows,width", [(2, 100), (16, 300)])
-def test_prefill_hidden_tokens_never_count(native_lib, device, rows, width):
+@pytest.mark.parametrize("rows,width,wide", [(2, 100, 0), (16, 300, 0), (2, 100, 200)])  # the last in parts
+def test_prefill_hidden_tokens_never_count(native_lib, device, rows, width, wide):
     """NaN in history slots past start_lens, unused blocks and the chunk's padding rows changes no bit."""
     starts = [70 - 3 * b for b in range(rows)]
     lens = [width - 11 * b for b in range(rows)]
     q, k, v, kp, vp, table = prefill_case(25, starts, lens, width, 4, 2)
+    table = np.pad(table, ((0, 0), (0, wide)))
     clean = run_prefill(device, (q, k, v, kp, vp, table), starts, lens)
     for pool, value in ((kp, False), (vp, True)):
         used = np.zeros((pool.shape[0], 16), dtype=bool)
