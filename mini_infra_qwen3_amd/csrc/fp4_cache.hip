@@ -14,7 +14,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kStoreTokens = kThreads / 16;  // tokens of a workgroup of the store
-constexpr int kGatherUnroll = 8;             // pieces of a thread in flight
+constexpr int kGatherHeads = 8;              // KV heads of a workgroup of the gather
 
 struct StoreArgs {
   const char* src[2][kMaxLayersPerLaunch];  // [0] keys, [1] values
@@ -125,32 +125,34 @@ struct GatherArgs {
   int64_t num_blocks;
   int32_t nb;
   int32_t kv_heads;
+  int32_t head_groups;  // ceil(kv_heads / kGatherHeads)
 };
 
-// One workgroup: one block of one table entry, K or V of one layer.  A block's output, [16 tokens][kv_heads]
-// [128] bf16, is contiguous: thread x writes its 16-byte pieces x, x + kThreads, ...
+// One workgroup: up to kGatherHeads KV heads of one block of one table entry, K or V of one layer.  Their records are
+// contiguous and go to LDS in whole 16-byte pieces; a row's 16 pieces of output are 16 lanes.
 __global__ __launch_bounds__(kThreads) void fp4_gather_kernel(const GatherArgs a) {
-  const int layer = blockIdx.y;
+  __shared__ __align__(16) unsigned char s_rec[kGatherHeads * kFp4Record];
+  const int layer = blockIdx.y / a.head_groups;
+  const int h0 = static_cast<int>(blockIdx.y % a.head_groups) * kGatherHeads;
+  const int heads = min(kGatherHeads, a.kv_heads - h0);
   const int c = blockIdx.z;
   const int64_t b = blockIdx.x / a.nb, j = blockIdx.x % a.nb;
   int64_t id = a.block_ids[b * a.block_id_stride + j];
   if (id < 0 || id >= a.num_blocks) id = 0;
-  const char* block = a.pool[c][layer] + id * a.kv_heads * kFp4Record;
-  u32x4* out = reinterpret_cast<u32x4*>(a.out[c][layer]) + static_cast<int64_t>(blockIdx.x) * kFp4Tokens * a.kv_heads * 16;
-  const int pieces = kFp4Tokens * 16 * a.kv_heads;  // a multiple of kThreads
-  for (int base = threadIdx.x; base < pieces; base += kThreads * kGatherUnroll) {
-    uint32_t codes[kGatherUnroll], scale[kGatherUnroll];
-#pragma unroll
-    for (int k = 0; k < kGatherUnroll; ++k) {
-      const int p = min(base + k * kThreads, pieces - 1);
-      const int octet = p & 15, h = (p >> 4) % a.kv_heads, t = (p >> 4) / a.kv_heads;
-      const char* rec = block + h * kFp4Record;
-      codes[k] = *reinterpret_cast<const uint32_t*>(rec + fp4_code_at(c == 1, t, octet));
-      scale[k] = *reinterpret_cast<const uint8_t*>(rec + fp4_scale_at(c == 1, t, octet));
-    }
-#pragma unroll
-    for (int k = 0; k < kGatherUnroll; ++k)
-      if (base + k * kThreads < pieces) store_stream<true>(out + base + k * kThreads, fp4_unpack8(codes[k], e8m0_f32(scale[k])));
+  const u32x4* block = reinterpret_cast<const u32x4*>(a.pool[c][layer] + (id * a.kv_heads + h0) * kFp4Record);
+  for (int x = threadIdx.x; x < heads * (kFp4Record / 16); x += kThreads)
+    reinterpret_cast<u32x4*>(s_rec)[x] = load_vec<true>(block + x);
+  __syncthreads();
+  char* out = a.out[c][layer] + (static_cast<int64_t>(blockIdx.x) * kFp4Tokens * a.kv_heads + h0) * (2 * kFp4Dim);
+  const int octet = threadIdx.x & 15;
+  for (int row = threadIdx.x >> 4; row < kFp4Tokens * heads; row += kThreads / 16) {
+    const int t = heads == kGatherHeads ? row / kGatherHeads : row / heads;
+    const int h = row - t * heads;
+    const unsigned char* rec = s_rec + h * kFp4Record;
+    const uint32_t codes = *reinterpret_cast<const uint32_t*>(rec + fp4_code_at(c == 1, t, octet));
+    const uint32_t scale = rec[fp4_scale_at(c == 1, t, octet)];
+    store_stream<true>(reinterpret_cast<u32x4*>(out + (static_cast<int64_t>(t) * a.kv_heads + h) * (2 * kFp4Dim)) + octet,
+                       fp4_unpack8(codes, e8m0_f32(scale)));
   }
 }
 
@@ -256,7 +258,7 @@ extern "C" int32_t mi_gather_blocks_fp4(const void* const* key_pools, const void
   if (block_id_stride < num_gathered_blocks)
     return fail(MI_ERR_INVALID_ARGUMENT, "%s: block_id_stride < num_gathered_blocks", name);
   const int64_t groups = static_cast<int64_t>(batch) * num_gathered_blocks;
-  if (groups > kMaxGroups || num_kv_heads > (1 << 20))
+  if (groups > kMaxGroups || num_kv_heads > 2048 * kGatherHeads)  // grid y: fewer than 65536
     return fail(MI_ERR_UNSUPPORTED, "%s: too many blocks", name);
   GatherArgs a{};
   a.block_ids = block_ids;
@@ -264,6 +266,7 @@ extern "C" int32_t mi_gather_blocks_fp4(const void* const* key_pools, const void
   a.num_blocks = num_blocks;
   a.nb = num_gathered_blocks;
   a.kv_heads = num_kv_heads;
+  a.head_groups = (num_kv_heads + kGatherHeads - 1) / kGatherHeads;
   for (int l = 0; l < num_layers; ++l) {
     if (!key_pools[l] || !value_pools[l] || !key_out[l] || !value_out[l])
       return fail(MI_ERR_INVALID_ARGUMENT, "%s: null pointer for layer %d", name, l);
@@ -278,7 +281,7 @@ extern "C" int32_t mi_gather_blocks_fp4(const void* const* key_pools, const void
       a.out[0][l] = static_cast<char*>(key_out[l0 + l]);
       a.out[1][l] = static_cast<char*>(value_out[l0 + l]);
     }
-    fp4_gather_kernel<<<dim3(static_cast<uint32_t>(groups), nl, 2), kThreads, 0, as_stream(stream)>>>(a);
+    fp4_gather_kernel<<<dim3(static_cast<uint32_t>(groups), nl * a.head_groups, 2), kThreads, 0, as_stream(stream)>>>(a);
     if (const int32_t rc = check_launch(name)) return rc;
   }
   return ok();
