@@ -849,11 +849,13 @@ def _record_pools(key_pools: Sequence[torch.Tensor], value_pools: Sequence[torch
     if len(key_pools) != len(value_pools) or not key_pools:
         raise ValueError("key_pools and value_pools must be equal-length, non-empty per-layer lists")
     pool0 = key_pools[0]
-    device = pool0.device
+    device, shape, dtype = pool0.device, pool0.shape, pool0.dtype
+    index = pool0.get_device()
     for name, tensors in (("key_pools", key_pools), ("value_pools", value_pools)):
         for t in tensors:
-            _require_gpu(name, t, device)
-            if t.shape != pool0.shape or t.dtype != pool0.dtype or not t.is_contiguous() or t.dim() != 4:
+            if index < 0 or t.get_device() != index:
+                _require_gpu(name, t, device)
+            if t.shape != shape or t.dtype is not dtype or not t.is_contiguous() or len(shape) != 4:
                 raise ValueError(f"{name}: expected contiguous {tuple(pool0.shape)} {pool0.dtype}, got "
                                  f"{tuple(t.shape)} {t.dtype}")
     block_bytes = pool0[0].numel() * pool0.element_size()
@@ -968,15 +970,18 @@ def fp4_pool_shape(num_blocks: int, block_size: int, num_kv_heads: int, head_dim
     return num_blocks, block_size // KERNEL_BLOCK_SIZE, num_kv_heads, FP4_RECORD_BYTES
 
 
-def _call(device: torch.device, name: str, *args) -> None:
-    """Calls an entry point with the tensors' device current (a launch goes to the current device's runtime state)."""
+def _on_device(device: torch.device, name: str, *args) -> int:
+    """An entry point's answer with the tensors' device current: a launch goes to the current device's runtime state,
+    and a workspace's size follows the current device's number of CUs."""
     entry = getattr(_native.load(), name)
     if torch._C._cuda_getDevice() == device.index:
-        rc = entry(*args)
-    else:
-        with torch.cuda.device(device):
-            rc = entry(*args)
-    _native.check(rc, name)
+        return entry(*args)
+    with torch.cuda.device(device):
+        return entry(*args)
+
+
+def _call(device: torch.device, name: str, *args) -> None:
+    _native.check(_on_device(device, name, *args), name)
 
 
 def _require_fp4_pools(key_pools: Sequence[torch.Tensor], value_pools: Sequence[torch.Tensor]) -> torch.Tensor:
@@ -1128,7 +1133,8 @@ def _workspace(workspace: torch.Tensor | None, need: int, device: torch.device) 
 
 def paged_decode_fp4_workspace_bytes(batch: int, max_blocks: int, num_heads: int, num_kv_heads: int,
                                      block_size: int = KERNEL_BLOCK_SIZE) -> int:
-    """Workspace for ``paged_decode_attention_fp4`` on ``[batch, max_blocks]`` tables (0: none needed)."""
+    """Workspace for ``paged_decode_attention_fp4`` on ``[batch, max_blocks]`` tables on the current device
+    (0: none needed)."""
     return int(_native.load().mi_paged_decode_fp4_workspace_bytes(
         batch, max_blocks * max(block_size // KERNEL_BLOCK_SIZE, 1), num_heads, num_kv_heads))
 
@@ -1179,7 +1185,7 @@ def paged_decode_attention_fp4(
         block_tables = block_tables.contiguous()
     if batch > 1 and context_lens.stride(0) <= 0:
         context_lens = context_lens.contiguous()
-    need = _native.load().mi_paged_decode_fp4_workspace_bytes(batch, max_blocks, num_heads, num_kv_heads)
+    need = _on_device(device, "mi_paged_decode_fp4_workspace_bytes", batch, max_blocks, num_heads, num_kv_heads)
     ws_ptr, ws_bytes, workspace = _workspace(workspace, need, device)
     _call(device, "mi_paged_decode_attention_fp4", out.data_ptr(), out.stride(0) if batch > 1 else num_heads * head_dim,
           query.data_ptr(), query.stride(0) if batch > 1 else num_heads * head_dim,
@@ -1192,7 +1198,8 @@ def paged_decode_attention_fp4(
 
 def chunked_prefill_fp4_workspace_bytes(batch: int, padded_len: int, num_heads: int, num_kv_heads: int, history_blocks: int,
                                         block_size: int = KERNEL_BLOCK_SIZE) -> int:
-    """Workspace for ``chunked_prefill_attention_fp4`` with tables of ``history_blocks`` (0: none needed)."""
+    """Workspace for ``chunked_prefill_attention_fp4`` with tables of ``history_blocks`` on the current device
+    (0: none needed)."""
     return int(_native.load().mi_chunked_prefill_fp4_workspace_bytes(
         batch, padded_len, num_heads, num_kv_heads, history_blocks * max(block_size // KERNEL_BLOCK_SIZE, 1)))
 
@@ -1252,7 +1259,7 @@ def chunked_prefill_attention_fp4(
         history_blocks = history_blocks.contiguous()
     if batch > 1 and (start_lens.stride(0) != chunk_lens.stride(0) or start_lens.stride(0) <= 0):
         start_lens, chunk_lens = start_lens.contiguous(), chunk_lens.contiguous()
-    need = _native.load().mi_chunked_prefill_fp4_workspace_bytes(batch, padded_len, num_heads, num_kv_heads, nb)
+    need = _on_device(device, "mi_chunked_prefill_fp4_workspace_bytes", batch, padded_len, num_heads, num_kv_heads, nb)
     ws_ptr, ws_bytes, workspace = _workspace(workspace, need, device)
 
     def strides(t):  # of a dim of one element any stride is good
