@@ -17,6 +17,11 @@ of Python containers:
   (``worker.block_tables.DeviceBlockTables``) stays current by uploading the deltas alone:
   one id per request whenever a decode step crosses a block boundary, instead of re-packing
   every table every step.
+
+Beyond the reference, a request can be forked (``KVCacheManager.fork``: the full blocks of the parent
+are shared and counted, the block that both would go on writing is copied) and the live blocks can be
+moved to the lowest ids (``KVCacheManager.compact``).  Both return block pairs for
+``PagedKVCachePool.copy_blocks``, which has to run before anything else writes those blocks.
 """
 
 from __future__ import annotations
@@ -114,6 +119,15 @@ class FreeKVCacheBlockQueue:
         self._count += n
         self.release_count += n
 
+    def relabel(self, old_ids: np.ndarray, new_ids: np.ndarray) -> None:
+        """Puts ``new_ids[i]`` in the place of the free id ``old_ids[i]``: the allocated block ``new_ids[i]`` has been
+        moved there.  The queue's order and counters stay (a moved-out block counts as the id it stands in for)."""
+        names = np.arange(self.num_blocks, dtype=np.int64)
+        names[old_ids] = new_ids
+        cap = self._ring.shape[0]
+        at = (self._head + np.arange(self._count)) % cap
+        self._ring[at] = names[self._ring[at]]
+
 
 class KVCacheManager:
     """Per-request block tables grown block by block. Reference block_manager.py:79-149.
@@ -133,6 +147,7 @@ class KVCacheManager:
         self._matrix = np.zeros((8, 8), dtype=np.int64)   # rows x blocks, null-padded
         self._blocks = np.zeros(8, dtype=np.int64)         # blocks per row
         self._tokens = np.zeros(8, dtype=np.int64)         # tokens per row
+        self._refs = np.zeros(num_blocks, dtype=np.int64)  # tables that hold a block
         self._rows_used = 0
         self._delta_rows: list[np.ndarray] = []
         self._delta_cols: list[np.ndarray] = []
@@ -219,26 +234,96 @@ class KVCacheManager:
             self._row_of[request_idx] = row
         if extra > 0:
             ids = np.asarray(self.free_block_queue.allocate(extra), dtype=np.int64)
-            end = have_blocks + extra
-            if end > self._matrix.shape[1]:
-                width = max(end, 2 * self._matrix.shape[1])
-                self._matrix = np.pad(self._matrix, ((0, 0), (0, width - self._matrix.shape[1])))
-            self._matrix[row, have_blocks:end] = ids
-            self._blocks[row] = end
-            self._delta_rows.append(np.full(extra, row, dtype=np.int64))
-            self._delta_cols.append(np.arange(have_blocks, end, dtype=np.int64))
-            self._delta_ids.append(ids)
+            self._refs[ids] = 1
+            self._write_table(row, have_blocks, ids)
         self._tokens[row] = total
         return True
 
+    def _write_table(self, row: int, column: int, ids: np.ndarray) -> None:
+        """Writes table entries ``[column, column + len(ids))``, the last of the row, and logs them."""
+        end = column + ids.shape[0]
+        if end > self._matrix.shape[1]:
+            width = max(end, 2 * self._matrix.shape[1])
+            self._matrix = np.pad(self._matrix, ((0, 0), (0, width - self._matrix.shape[1])))
+        self._matrix[row, column:end] = ids
+        self._blocks[row] = end
+        self._log(np.full(ids.shape[0], row, dtype=np.int64), np.arange(column, end, dtype=np.int64), ids)
+
+    def _log(self, rows: np.ndarray, cols: np.ndarray, ids: np.ndarray) -> None:
+        self._delta_rows.append(rows)
+        self._delta_cols.append(cols)
+        self._delta_ids.append(ids)
+
     def free(self, request_idx: int) -> None:
-        """Returns every block of the request to the free queue and its row to the spare rows."""
+        """Returns the request's blocks to the free queue, those that no other table holds, and its row to the spare rows."""
         row = self._row_of.pop(request_idx)
-        n = int(self._blocks[row])
-        self.free_block_queue.free(self._matrix[row, :n].copy())
+        ids = self._matrix[row, :int(self._blocks[row])].copy()
+        self._refs[ids] -= 1
+        self.free_block_queue.free(ids[self._refs[ids] == 0])
         self._blocks[row] = 0
         self._tokens[row] = 0
         self._spare_rows.append(row)
+
+    # -- forks and compaction (not in the reference) ------------------------------------------
+    def fork(self, parent_idx: int, child_idx: int, num_tokens: int | None = None) -> list[tuple[int, int]] | None:
+        """Starts request ``child_idx`` with the parent's first ``num_tokens`` tokens (default: all of them).
+
+        Their K/V must be in the pool already.  Full blocks are shared: nobody writes them again, and each goes back to
+        the free queue with its last holder.  A block that the tokens fill in part is copied, so that parent and child
+        each go on in their own.  Returns the ``(source, destination)`` pairs to copy (none or one), or None, without a
+        trace, when the copy finds no free block.
+        """
+        parent = self._row_of[parent_idx]
+        if child_idx in self._row_of:
+            raise ValueError(f"request {child_idx} has a block table already")
+        have = int(self._tokens[parent])
+        tokens = have if num_tokens is None else int(num_tokens)
+        if not 0 <= tokens <= have:
+            raise ValueError(f"request {parent_idx} has {have} tokens, cannot fork {tokens}")
+        full, rest = divmod(tokens, self.block_size)
+        if rest and self.free_block_queue.num_free_blocks < 1:
+            return None
+        ids = self._matrix[parent, :full + (rest > 0)].copy()
+        self._refs[ids[:full]] += 1
+        pairs = []
+        if rest:
+            own = self.free_block_queue.allocate(1)[0]
+            self._refs[own] = 1
+            pairs.append((int(ids[full]), own))
+            ids[full] = own
+        row = self._row_of[child_idx] = self._new_row()
+        if ids.shape[0]:
+            self._write_table(row, 0, ids)
+        self._tokens[row] = tokens
+        return pairs
+
+    def compact(self) -> list[tuple[int, int]]:
+        """Gives the ``n`` blocks in use the ids ``1..n``: those above move to the free ids below.
+
+        Tables (and their deltas) and the free queue are up to date on return.  Returns the ``(source, destination)``
+        pairs; no destination is a source, and the copy has to be enqueued before the next step.
+        """
+        live = np.flatnonzero(self._refs)
+        n = live.shape[0]
+        if n != self.num_used_blocks:
+            raise RuntimeError(f"{self.num_used_blocks} blocks are in use, tables hold {n}: compact() moves only blocks "
+                               "of this manager's tables")
+        src = live[live > n]
+        if src.shape[0] == 0:
+            return []
+        dst = 1 + np.flatnonzero(self._refs[1:n + 1] == 0)
+        moved = np.arange(self._refs.shape[0], dtype=np.int64)
+        moved[src] = dst
+        for row in self._row_of.values():
+            ids = self._matrix[row, :int(self._blocks[row])]
+            cols = np.flatnonzero(moved[ids] != ids)
+            if cols.shape[0]:
+                ids[cols] = moved[ids[cols]]  # a view: the matrix itself
+                self._log(np.full(cols.shape[0], row, dtype=np.int64), cols, ids[cols])
+        self._refs[dst] = self._refs[src]
+        self._refs[src] = 0
+        self.free_block_queue.relabel(dst, src)
+        return list(zip(src.tolist(), dst.tolist()))
 
 
 __all__ = [

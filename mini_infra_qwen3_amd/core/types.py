@@ -34,17 +34,23 @@ class PagedCacheConfig:
     """Paged KV cache settings. Reference src/mini_infra/core/types.py:47-66.
 
     block_size: tokens per block; num_blocks: pool size including the null block (None: derive
-    it from the workload with ``required_pool_blocks``).
+    it from the workload with ``required_pool_blocks``).  kv_bits (not in the reference): 16, the model's
+    dtype, or 4, the 4-bit pool (``PagedKVCachePoolFp4``: block_size a multiple of 16).
     """
 
     block_size: int = 16
     num_blocks: int | None = None
+    kv_bits: int = 16
 
     def __post_init__(self) -> None:
         if self.block_size < 1:
             raise ValueError("block_size must be positive")
         if self.num_blocks is not None and self.num_blocks < 2:
             raise ValueError("num_blocks must be at least 2 (block 0 is the null block)")
+        if self.kv_bits not in (4, 16):
+            raise ValueError(f"kv_bits must be 16 or 4, got {self.kv_bits}")
+        if self.kv_bits == 4 and self.block_size % 16 != 0:
+            raise ValueError(f"4-bit pools need a block_size that is a multiple of 16, got {self.block_size}")
 
 
 __all__ = ["PagedCacheConfig", "Request"]

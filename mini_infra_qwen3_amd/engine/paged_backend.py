@@ -26,7 +26,7 @@ from mini_infra_qwen3_amd.core import KVCacheManager, PagedCacheConfig, num_bloc
 from mini_infra_qwen3_amd.core.scheduler import PrefillChunk, RequestState
 from mini_infra_qwen3_amd.core.types import Request
 from mini_infra_qwen3_amd.device import synchronize
-from mini_infra_qwen3_amd.worker import PagedKVCachePool, PagedRunner
+from mini_infra_qwen3_amd.worker import PagedKVCachePool, PagedKVCachePoolFp4, PagedRunner
 from mini_infra_qwen3_amd.worker.block_tables import DeviceBlockTables
 
 
@@ -58,7 +58,8 @@ class PagedScheduleBackend:
         tokens in all: the scheduler's token budget, or no cap) with up to ``mixed_graph_decode_rows``
         decode rows.  A model with reference numerics (``exact``) takes decode graphs per batch size,
         mixed graphs at the padded shapes it runs every mixed step at (``padded_mixed_shape``) and
-        no prefill graphs (they pad the chunk width: ValueError)."""
+        no prefill graphs (they pad the chunk width: ValueError).  ``paged_cache_config.kv_bits`` 4: a 4-bit
+        pool, for models without reference numerics."""
         self.model = model
         self.device = next(model.parameters()).device
         self.block_size = paged_cache_config.block_size
@@ -70,9 +71,13 @@ class PagedScheduleBackend:
                              "(plus the null block)")
         config = model.config
         self.runner = PagedRunner(model, pad_token_id)
-        self.pool = PagedKVCachePool(config.num_hidden_layers, num_blocks, self.block_size,
-                                     config.num_key_value_heads, config.head_dim,
-                                     next(model.parameters()).dtype, self.device)
+        geometry = (config.num_hidden_layers, num_blocks, self.block_size, config.num_key_value_heads, config.head_dim)
+        if paged_cache_config.kv_bits == 4:
+            if getattr(model, "exact", False):
+                raise ValueError("a 4-bit pool has no reference numerics: its model needs exact=False")
+            self.pool = PagedKVCachePoolFp4(*geometry, self.device)
+        else:
+            self.pool = PagedKVCachePool(*geometry, next(model.parameters()).dtype, self.device)
         self.kv_cache_manager = KVCacheManager(self.block_size, num_blocks)
         self.tables = DeviceBlockTables(self.kv_cache_manager, min(max_running_requests, len(requests)), largest,
                                         self.device)
@@ -93,6 +98,13 @@ class PagedScheduleBackend:
 
     def _live_bytes(self) -> int:
         return self.kv_cache_manager.num_used_blocks * self.pool.bytes_per_block
+
+    def compact_cache(self) -> int:
+        """Moves the live blocks to the lowest ids of the pool (one launch); returns how many moved."""
+        pairs = self.kv_cache_manager.compact()
+        if pairs:
+            self.pool.copy_blocks([s for s, _ in pairs], [d for _, d in pairs])
+        return len(pairs)
 
     def execute_prefill(self, chunks: Sequence[PrefillChunk]) -> ScheduleStepOutput:
         tables = [self.kv_cache_manager.block_table(c.state.request.request_idx) for c in chunks]

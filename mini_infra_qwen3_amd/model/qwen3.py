@@ -16,6 +16,8 @@ state_dict loads unchanged.  The attention differs in how it reaches K/V:
   run once over all tokens; q/k norm + RoPE and attention run in their prefill and decode forms
   on the two token ranges, writing one output buffer.
 
+Pools of 4 bits (``PagedKVCachePoolFp4``) serve all three, without reference numerics.
+
 Dense GEMMs (projections, MLP, lm_head) stay on PyTorch-ROCm; the elementwise chains around them
 run as fused launches of the same library (``data_plane.rms_norm`` with the residual add,
 ``qk_norm_rope`` with the decode append, ``silu_mul``), keeping the reference's bf16 rounding points.
@@ -194,6 +196,8 @@ class Qwen3Attention(nn.Module):
             q, k, v = qkv[..., :nq], qkv[..., nq:nq + nkv], qkv[..., nq + nkv:]
         key_pool, value_pool = kv_pool
         eps = self.q_norm.eps
+        if key_pool.dtype is torch.uint8:
+            return self._fp4(q, k, v, cos, sin, kv_pool, metadata, workspace, kv_out)
         if isinstance(metadata, PagedMixedMetadata):
             return self._mixed(q[0], k[0], v[0], cos[0], sin[0], kv_pool, metadata, workspace, kv_out)
         if isinstance(metadata, PagedAttentionMetadata):
@@ -220,6 +224,63 @@ class Qwen3Attention(nn.Module):
             )
             present = (k_rot, v_rows)
         return self.o_proj(out), present
+
+    def _fp4(self, q, k, v, cos, sin, kv_pool: PastKeyValue, metadata, workspace, kv_out=None):
+        """The three forms of ``forward`` on a 4-bit pool: q/k norm + RoPE, the store of the rows that have a slot, then
+        attention, a launch each (two more than the fused decode of 16-bit pools, whose append is part of the norm's).
+        A decoding token sees its own K/V as stored, in 4 bits; a chunk sees itself in bf16 and its history in 4 bits.
+
+        A mixed step's chunk rows are laid out left-padded for the prefill kernel (one gather each of q, k and v, one
+        scatter of the output)."""
+        key_pool, value_pool = kv_pool
+        heads, kv_heads, dim = self.num_heads, self.num_kv_heads, self.head_dim
+        batch, length = q.shape[:2]
+        k_buf, v_buf = kv_out if kv_out is not None else (None, None)
+        q_rot, k_rot, v_rows = data_plane.qk_norm_rope(q, k, v, self.q_norm.weight, self.k_norm.weight, cos, sin,
+                                                       self.q_norm.eps, k_out=k_buf, v_out=v_buf)
+
+        def store(first: int, slots):  # tokens [first, first + len(slots)), as rows of one token
+            n = slots.shape[0]
+            data_plane.reshape_and_cache_fp4([k_rot[first:first + n].unsqueeze(2)], [v_rows[first:first + n].unsqueeze(2)],
+                                             slots, [key_pool], [value_pool])
+
+        def decode(first: int, meta: PagedAttentionMetadata, out=None):
+            store(first, meta.slot_mapping)
+            return data_plane.paged_decode_attention_fp4(
+                q_rot[first:first + meta.slot_mapping.shape[0]], key_pool, value_pool, meta.block_tables,
+                meta.context_lens, self.scaling, out=out, workspace=workspace)
+
+        def prefill(q_rows, k_rows, v_rows, meta: PagedPrefillMetadata):  # [B, L, H, D] each
+            return data_plane.chunked_prefill_attention_fp4(
+                q_rows.transpose(1, 2), k_rows.transpose(1, 2), v_rows.transpose(1, 2), key_pool, value_pool,
+                meta.history_block_tables, meta.start_lens, meta.chunk_lens, self.scaling, workspace=workspace)
+
+        if isinstance(metadata, PagedAttentionMetadata):
+            return self.o_proj(decode(0, metadata).view(batch, 1, -1)), kv_pool
+        if isinstance(metadata, PagedPrefillMetadata):
+            if metadata.slot_mapping is not None:
+                store(0, metadata.slot_mapping.reshape(-1))
+            k_seq, v_seq = k_rot.view(batch, length, kv_heads, dim), v_rows.view(batch, length, kv_heads, dim)
+            out = prefill(q_rot.view(batch, length, heads, dim), k_seq, v_seq, metadata)
+            return self.o_proj(out), (k_seq.transpose(1, 2), v_seq.transpose(1, 2))
+        rows, width, n = metadata.prefill_rows, metadata.prefill_width, metadata.chunk_span
+        out = torch.zeros((length + 1, heads * dim), dtype=q_rot.dtype, device=q_rot.device)  # the last row: padding
+        decode(n, metadata.decode, out=out[n:length])
+        if metadata.chunk_first is None:
+            out[:n] = prefill(q_rot[:n].view(rows, width, heads, dim), k_rot[:n].view(rows, width, kv_heads, dim),
+                              v_rows[:n].view(rows, width, kv_heads, dim), metadata.prefill).view(n, -1)
+            per_row = (rows, width)
+        else:
+            lens = metadata.prefill.chunk_lens.clamp(0, min(width, n)).unsqueeze(1)
+            first = torch.minimum(metadata.chunk_first.unsqueeze(1).clamp(min=0), n - lens)
+            ahead = torch.arange(width, device=q_rot.device) - (width - lens)  # token of the row, negative in its padding
+            token = torch.where(ahead >= 0, first + ahead, 0).reshape(-1)
+            chunk = [t.index_select(0, token).view(rows, width, *t.shape[1:]) for t in (q_rot, k_rot, v_rows)]
+            padded = prefill(*chunk, metadata.prefill).view(rows * width, -1)
+            out.index_copy_(0, torch.where(ahead.reshape(-1) >= 0, token, length), padded)
+            per_row = (1, n)
+        present = tuple(t[:n].view(*per_row, kv_heads, dim).transpose(1, 2) for t in (k_rot, v_rows))
+        return self.o_proj(out[:length].unsqueeze(0)), present
 
     def _mixed(self, q, k, v, cos, sin, kv_pool: PastKeyValue, metadata: PagedMixedMetadata, workspace, kv_out=None):
         """One q/k norm + RoPE launch over all T tokens, then one attention launch for the chunk rows
@@ -292,6 +353,24 @@ class Qwen3Model(nn.Module):
             "_empty_pool", torch.zeros(1, 16, config.num_key_value_heads, config.head_dim), persistent=False
         )
 
+    def _fp4_pools(self, pools) -> bool:
+        """Whether the pools are 4-bit ones, which a model with reference numerics refuses."""
+        if len(pools) == 0 or pools[0][0].dtype is not torch.uint8:
+            return False
+        if any(layer.self_attn.exact for layer in self.layers):
+            raise ValueError("a 4-bit pool has no reference numerics: its model needs exact=False")
+        return True
+
+    def _fp4_decode_bytes(self, rows: int, tables: torch.Tensor, pools) -> int:
+        return data_plane.paged_decode_fp4_workspace_bytes(rows, tables.shape[1], self.config.num_attention_heads,
+                                                           self.config.num_key_value_heads,
+                                                           data_plane.KERNEL_BLOCK_SIZE * pools[0][0].shape[1])
+
+    def _fp4_prefill_bytes(self, rows: int, width: int, tables: torch.Tensor, pools) -> int:
+        return data_plane.chunked_prefill_fp4_workspace_bytes(rows, width, self.config.num_attention_heads,
+                                                              self.config.num_key_value_heads, tables.shape[1],
+                                                              data_plane.KERNEL_BLOCK_SIZE * pools[0][0].shape[1])
+
     def forward(self, input_ids: torch.Tensor, attention_mask: torch.Tensor | None = None,
                 position_ids: torch.Tensor | None = None,
                 attn_metadata: PagedAttentionMetadata | PagedPrefillMetadata | PagedMixedMetadata | None = None,
@@ -322,9 +401,13 @@ class Qwen3Model(nn.Module):
                 raise ValueError("a mixed step needs position_ids")
             if len(pools) != len(self.layers):
                 raise ValueError("kv_pools has a different number of layers than the model")
-            need = data_plane.paged_decode_workspace_bytes(decode_rows, metadata.decode.block_tables.shape[1],
-                                                          self.config.num_attention_heads, self.config.head_dim,
-                                                          pools[0][0].shape[1], self.config.num_key_value_heads)
+            if self._fp4_pools(pools):
+                need = max(self._fp4_decode_bytes(decode_rows, metadata.decode.block_tables, pools),
+                           self._fp4_prefill_bytes(rows, metadata.prefill_width, metadata.prefill.history_block_tables, pools))
+            else:
+                need = data_plane.paged_decode_workspace_bytes(decode_rows, metadata.decode.block_tables.shape[1],
+                                                              self.config.num_attention_heads, self.config.head_dim,
+                                                              pools[0][0].shape[1], self.config.num_key_value_heads)
             if need:
                 workspace = torch.empty(need, dtype=torch.uint8, device=device)
         elif isinstance(attn_metadata, PagedAttentionMetadata):
@@ -339,15 +422,18 @@ class Qwen3Model(nn.Module):
                 metadata = metadata._replace(block_tables=metadata.block_tables.index_select(0, metadata.table_rows),
                                              table_rows=None)
             pools = attn_metadata.kv_pools
-            # one buffer serves either decode form: the bandwidth kernel's split-context partials or
-            # the reference-numerics kernel's split form
-            need = max(data_plane.paged_decode_workspace_bytes(batch, metadata.block_tables.shape[1],
-                                                              self.config.num_attention_heads, self.config.head_dim,
-                                                              pools[0][0].shape[1], self.config.num_key_value_heads),
-                       data_plane.paged_decode_exact_workspace_bytes(batch, metadata.block_tables.shape[1],
-                                                                     self.config.num_attention_heads,
-                                                                     self.config.num_key_value_heads,
-                                                                     pools[0][0].shape[1]))
+            if self._fp4_pools(pools):
+                need = self._fp4_decode_bytes(batch, metadata.block_tables, pools)
+            else:
+                # one buffer serves either decode form: the bandwidth kernel's split-context partials or
+                # the reference-numerics kernel's split form
+                need = max(data_plane.paged_decode_workspace_bytes(batch, metadata.block_tables.shape[1],
+                                                                  self.config.num_attention_heads, self.config.head_dim,
+                                                                  pools[0][0].shape[1], self.config.num_key_value_heads),
+                           data_plane.paged_decode_exact_workspace_bytes(batch, metadata.block_tables.shape[1],
+                                                                         self.config.num_attention_heads,
+                                                                         self.config.num_key_value_heads,
+                                                                         pools[0][0].shape[1]))
             if need:
                 workspace = torch.empty(need, dtype=torch.uint8, device=device)
         else:
@@ -365,6 +451,10 @@ class Qwen3Model(nn.Module):
                 pools = attn_metadata.kv_pools
                 if len(pools) != len(self.layers):
                     raise ValueError("kv_pools has a different number of layers than the model")
+                if self._fp4_pools(pools):
+                    need = self._fp4_prefill_bytes(batch, length, metadata.history_block_tables, pools)
+                    if need:
+                        workspace = torch.empty(need, dtype=torch.uint8, device=device)
             else:
                 raise NotImplementedError(f"{type(attn_metadata).__name__}: only the paged path is built here")
             if position_ids is None:  # real tokens count from start, left padding sits at position 0

@@ -21,7 +21,7 @@ HBM and ``mi_unpack_blocks`` scatters records into (possibly other) blocks, so t
      20  I   block_size               60  I  reserved (0)
      24  I   num_kv_heads
      28  I   head_dim
-     32  I   dtype code (1 bf16, 2 fp16, 3 fp32)
+     32  I   dtype code (1 bf16, 2 fp16, 3 fp32, 4: 4-bit pool, records of bytes)
 
 Every call runs on the current stream.  Host memory of a swap-out is valid after that stream has
 passed it (``HostSwapPool.synchronize``); device blocks freed after a swap-out or a swap-in can be
@@ -40,11 +40,13 @@ from pathlib import Path
 
 import torch
 
+from mini_infra_qwen3_amd.data_plane import fp4_pool_shape
+
 RECORD_MAGIC = b"MIKVBLK1"
 FORMAT_VERSION = 1
 _HEADER = struct.Struct("<8sIIIIIIIIQQII")
 HEADER_BYTES = _HEADER.size  # 64
-DTYPE_CODES = {torch.bfloat16: 1, torch.float16: 2, torch.float32: 3}
+DTYPE_CODES = {torch.bfloat16: 1, torch.float16: 2, torch.float32: 3, torch.uint8: 4}
 _CODE_DTYPES = {code: dtype for dtype, code in DTYPE_CODES.items()}
 
 
@@ -66,10 +68,12 @@ class KVBlockHeader:
 
     @property
     def record_bytes(self) -> int:
-        return 2 * self.num_layers * self.block_size * self.num_kv_heads * self.head_dim * self.element_bytes
+        return math.prod(self.record_shape) * self.element_bytes
 
     @property
     def record_shape(self) -> tuple[int, ...]:
+        if self.dtype == torch.uint8:  # 16 tokens of a head to a piece of codes and scales
+            return (self.num_layers, 2, *fp4_pool_shape(1, self.block_size, self.num_kv_heads, self.head_dim)[1:])
         return (self.num_layers, 2, self.block_size, self.num_kv_heads, self.head_dim)
 
     def encode(self) -> bytes:
@@ -99,7 +103,7 @@ class KVBlockHeader:
 
 
 def pool_header(pool, num_records: int, crc32: int = 0) -> KVBlockHeader:
-    """Header describing records of ``pool`` (a PagedKVCachePool)."""
+    """Header describing records of ``pool`` (a PagedKVCachePool or PagedKVCachePoolFp4)."""
     return KVBlockHeader(len(pool.kv_pools), pool.block_size, pool.num_kv_heads, pool.head_dim, pool.storage.dtype,
                          num_records, crc32)
 

@@ -9,6 +9,8 @@ MI355X layout: all layers live in ONE allocation ``[num_layers, 2, num_blocks, b
 90 GB pool is a single HBM3E range), and ``kv_pools`` are views of it, so the per-layer tensors
 the reference's callers index are unchanged.  ``gather_blocks`` and ``write_prefill`` are single
 HIP launches over all layers (kernels 2 and 1) instead of per-layer advanced indexing.
+
+``PagedKVCachePoolFp4`` holds the same blocks in 4 bits (17/64 of the bf16 bytes), with the same calls.
 """
 
 from __future__ import annotations
@@ -51,6 +53,11 @@ class PagedKVCachePool:
         ]
 
     @property
+    def row_dtype(self) -> torch.dtype:
+        """dtype of the K/V rows that go in and come out."""
+        return self.storage.dtype
+
+    @property
     def device(self) -> torch.device:
         return self.storage.device
 
@@ -73,6 +80,9 @@ class PagedKVCachePool:
         ``transpose(1, 2)`` views of a contiguous ``[B, nb * block_size, H_kv, D]`` gather, exactly
         as the reference returns them (whole blocks, null block and stale tails included).
         """
+        return self._gather(block_ids, data_plane.gather_blocks)
+
+    def _gather(self, block_ids: torch.Tensor, gather) -> tuple[tuple[torch.Tensor, torch.Tensor], ...]:
         if block_ids.ndim != 2:
             raise ValueError(f"block_ids must be [batch, num_blocks], got {tuple(block_ids.shape)}")
         block_ids = block_ids.to(device=self.device, dtype=torch.long)
@@ -80,11 +90,11 @@ class PagedKVCachePool:
         num_layers = len(self.kv_pools)
         out = torch.empty(
             (num_layers, 2, batch, nb * self.block_size, self.num_kv_heads, self.head_dim),
-            dtype=self.storage.dtype, device=self.device,
+            dtype=self.row_dtype, device=self.device,
         )
         keys = [out[layer, 0] for layer in range(num_layers)]
         values = [out[layer, 1] for layer in range(num_layers)]
-        data_plane.gather_blocks(
+        gather(
             [k for k, _ in self.kv_pools], [v for _, v in self.kv_pools], block_ids, keys, values
         )
         return tuple((k.transpose(1, 2), v.transpose(1, 2)) for k, v in zip(keys, values))
@@ -110,6 +120,19 @@ class PagedKVCachePool:
         data_plane.unpack_blocks(records, [k for k, _ in self.kv_pools], [v for _, v in self.kv_pools],
                                  self._block_id_tensor(block_ids, unique=True))
 
+    def copy_blocks(self, src_blocks, dst_blocks) -> None:
+        """Block ``dst_blocks[i]`` of every layer becomes block ``src_blocks[i]``, K and V, in one kernel launch on the
+        current stream (for ``KVCacheManager.fork`` and ``compact``).
+
+        Destinations are unique and none is a source; lists are checked, tensors are taken as they are.
+        """
+        if not isinstance(src_blocks, torch.Tensor) and not isinstance(dst_blocks, torch.Tensor):
+            if set(map(int, src_blocks)) & set(map(int, dst_blocks)):
+                raise ValueError("a block that one call writes cannot be its source as well")
+        src = self._block_id_tensor(src_blocks, unique=False)
+        dst = self._block_id_tensor(dst_blocks, unique=True)
+        data_plane.copy_blocks([k for k, _ in self.kv_pools], [v for _, v in self.kv_pools], src, dst)
+
     def write_prefill(
         self,
         prefill_cache: KVCache,
@@ -122,10 +145,14 @@ class PagedKVCachePool:
         prefill_cache: per layer ``(key, value)``, each ``[B, H_kv, L, D]`` (any strides, D contiguous).
         token_rows / token_positions / slot_mapping: ``[N]`` int64; slots must be unique.
         """
+        self._write(prefill_cache, token_rows, token_positions, slot_mapping, data_plane.reshape_and_cache)
+
+    def _write(self, prefill_cache: KVCache, token_rows: torch.Tensor, token_positions: torch.Tensor,
+               slot_mapping: torch.Tensor, scatter) -> None:
         caches = list(prefill_cache)
         if len(caches) != len(self.kv_pools):
             raise ValueError(f"prefill_cache has {len(caches)} layers, pool has {len(self.kv_pools)}")
-        data_plane.reshape_and_cache(
+        scatter(
             [k for k, _ in caches],
             [v for _, v in caches],
             slot_mapping,
@@ -136,4 +163,43 @@ class PagedKVCachePool:
         )
 
 
-__all__ = ["PagedKVCachePool"]
+class PagedKVCachePoolFp4(PagedKVCachePool):
+    """A ``PagedKVCachePool`` in 4 bits (MXFP4, ``data_plane.fp4_pool_shape``): groups of 32 dims with a
+    power-of-two scale byte, 4.25 bits a value, so a block takes 17/64 of its bf16 bytes.
+
+    ``kv_pools[layer]``: (key, value) pools, uint8 ``[num_blocks, block_size / 16, H_kv, 1088]``.  K/V rows are
+    quantised when they are written (bf16, fp16 or fp32) and come back as the bf16 values that they stand for; the
+    attention kernels read the pool as it is.  Block records are its bytes: pools of one geometry exchange blocks
+    exactly.
+    """
+
+    def __init__(self, num_layers: int, num_blocks: int, block_size: int, num_kv_heads: int, head_dim: int,
+                 device: torch.device | str):
+        device = torch.device(device)
+        if device.type != "cuda":
+            raise RuntimeError(f"PagedKVCachePoolFp4 needs a GPU device, got {device} (no CPU data plane)")
+        if num_layers < 1 or num_blocks < 1:
+            raise ValueError("PagedKVCachePoolFp4: every dimension must be positive")
+        shape = data_plane.fp4_pool_shape(num_blocks, block_size, num_kv_heads, head_dim)
+        self.num_blocks = num_blocks
+        self.block_size = block_size
+        self.num_kv_heads = num_kv_heads
+        self.head_dim = head_dim
+        self.storage = torch.zeros((num_layers, 2, *shape), dtype=torch.uint8, device=device)
+        self.kv_pools = [(self.storage[layer, 0], self.storage[layer, 1]) for layer in range(num_layers)]
+
+    @property
+    def row_dtype(self) -> torch.dtype:
+        return torch.bfloat16
+
+    def gather_blocks(self, block_ids: torch.Tensor) -> tuple[tuple[torch.Tensor, torch.Tensor], ...]:
+        """``PagedKVCachePool.gather_blocks``, the values as bf16."""
+        return self._gather(block_ids, data_plane.gather_blocks_fp4)
+
+    def write_prefill(self, prefill_cache: KVCache, token_rows: torch.Tensor, token_positions: torch.Tensor,
+                      slot_mapping: torch.Tensor) -> None:
+        """``PagedKVCachePool.write_prefill``, quantising."""
+        self._write(prefill_cache, token_rows, token_positions, slot_mapping, data_plane.reshape_and_cache_fp4)
+
+
+__all__ = ["PagedKVCachePool", "PagedKVCachePoolFp4"]

@@ -252,7 +252,7 @@ class PagedRunner(BaseModelRunner):
         if self._staging is None or self._staging.shape[2] < tokens:
             cfg = self.model.config
             self._staging = torch.empty((cfg.num_hidden_layers, 2, tokens, cfg.num_key_value_heads, cfg.head_dim),
-                                        dtype=pool.storage.dtype, device=self.device)
+                                        dtype=pool.row_dtype, device=self.device)
         if self._mempool is None:
             self._mempool = torch.cuda.graph_pool_handle()
         return self._staging
