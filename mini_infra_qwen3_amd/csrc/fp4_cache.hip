@@ -14,6 +14,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kStoreTokens = kThreads / 16;  // tokens of a workgroup of the store
+constexpr int kGatherThreads = 512;
 constexpr int kGatherHeads = 8;              // KV heads of a workgroup of the gather
 
 struct StoreArgs {
@@ -74,6 +75,11 @@ __device__ __forceinline__ void load8(float (&x)[8], const char* p) {
 // One workgroup: kStoreTokens index entries of one KV head of one layer, K and V.  A wavefront's four rows are
 // four entries; where they are the tokens of a quad of one block (a prompt's store), its V codes are 256
 // contiguous bytes.
+//
+// Bound by memory: 3614 tokens of four prompts, 28 layers of 8 heads (525 MB) in 105 us, 5.0 TB/s.  How the work is laid out
+// moves little: 2 or 4 layers a workgroup, a record's neighbours kept on one XCD, 128 to 1024 threads 101 to 110; K and V
+// in workgroups of their own 125.  Ordinary loads take 112, nontemporal stores 124 (a record's lines are filled by several
+// wavefronts, which the L2 joins).
 template <Source kType, bool kWide>
 __global__ __launch_bounds__(kThreads) void fp4_store_kernel(const StoreArgs a) {
   const int h = static_cast<int>(blockIdx.x % a.kv_heads);
@@ -130,7 +136,12 @@ struct GatherArgs {
 
 // One workgroup: up to kGatherHeads KV heads of one block of one table entry, K or V of one layer.  Their records are
 // contiguous and go to LDS in whole 16-byte pieces; a row's 16 pieces of output are 16 lanes.
-__global__ __launch_bounds__(kThreads) void fp4_gather_kernel(const GatherArgs a) {
+//
+// Bound by memory: 1.75 GB (28 layers, 32 sequences of up to 1150 tokens, 8 heads) in 262 us, 6.7 TB/s, what a plain copy
+// reaches; without LDS, a lane reading its own four code bytes, 422.  256 threads 291, and 315 with nontemporal loads (a
+// record's second half is a line of its neighbour's); 4 heads a workgroup as fast here, but 12.2 us against 11.5 for one
+// sequence of 1024 tokens; ordinary stores 359 against 315, nontemporal ones without sc1 335.
+__global__ __launch_bounds__(kGatherThreads) void fp4_gather_kernel(const GatherArgs a) {
   __shared__ __align__(16) unsigned char s_rec[kGatherHeads * kFp4Record];
   const int layer = blockIdx.y / a.head_groups;
   const int h0 = static_cast<int>(blockIdx.y % a.head_groups) * kGatherHeads;
@@ -140,12 +151,12 @@ __global__ __launch_bounds__(kThreads) void fp4_gather_kernel(const GatherArgs a
   int64_t id = a.block_ids[b * a.block_id_stride + j];
   if (id < 0 || id >= a.num_blocks) id = 0;
   const u32x4* block = reinterpret_cast<const u32x4*>(a.pool[c][layer] + (id * a.kv_heads + h0) * kFp4Record);
-  for (int x = threadIdx.x; x < heads * (kFp4Record / 16); x += kThreads)
-    reinterpret_cast<u32x4*>(s_rec)[x] = load_vec<true>(block + x);
+  for (int x = threadIdx.x; x < heads * (kFp4Record / 16); x += kGatherThreads)
+    reinterpret_cast<u32x4*>(s_rec)[x] = block[x];
   __syncthreads();
   char* out = a.out[c][layer] + (static_cast<int64_t>(blockIdx.x) * kFp4Tokens * a.kv_heads + h0) * (2 * kFp4Dim);
   const int octet = threadIdx.x & 15;
-  for (int row = threadIdx.x >> 4; row < kFp4Tokens * heads; row += kThreads / 16) {
+  for (int row = threadIdx.x >> 4; row < kFp4Tokens * heads; row += kGatherThreads / 16) {
     const int t = heads == kGatherHeads ? row / kGatherHeads : row / heads;
     const int h = row - t * heads;
     const unsigned char* rec = s_rec + h * kFp4Record;
@@ -258,7 +269,7 @@ extern "C" int32_t mi_gather_blocks_fp4(const void* const* key_pools, const void
   if (block_id_stride < num_gathered_blocks)
     return fail(MI_ERR_INVALID_ARGUMENT, "%s: block_id_stride < num_gathered_blocks", name);
   const int64_t groups = static_cast<int64_t>(batch) * num_gathered_blocks;
-  if (groups > kMaxGroups || num_kv_heads > 2048 * kGatherHeads)  // grid y: fewer than 65536
+  if (groups > 0xffffffffll / kGatherThreads || num_kv_heads > 2048 * kGatherHeads)  // grid y: fewer than 65536
     return fail(MI_ERR_UNSUPPORTED, "%s: too many blocks", name);
   GatherArgs a{};
   a.block_ids = block_ids;
@@ -281,7 +292,7 @@ extern "C" int32_t mi_gather_blocks_fp4(const void* const* key_pools, const void
       a.out[0][l] = static_cast<char*>(key_out[l0 + l]);
       a.out[1][l] = static_cast<char*>(value_out[l0 + l]);
     }
-    fp4_gather_kernel<<<dim3(static_cast<uint32_t>(groups), nl * a.head_groups, 2), kThreads, 0, as_stream(stream)>>>(a);
+    fp4_gather_kernel<<<dim3(static_cast<uint32_t>(groups), nl * a.head_groups, 2), kGatherThreads, 0, as_stream(stream)>>>(a);
     if (const int32_t rc = check_launch(name)) return rc;
   }
   return ok();

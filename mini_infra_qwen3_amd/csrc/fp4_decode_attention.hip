@@ -6,13 +6,15 @@
 // reference's gather, mask and attend: src/mini_infra/model/qwen3.py:219-292) for 136 bytes a token and KV head
 // instead of 512.  At that size a bf16 kernel's arithmetic would be the bound, so none is spent on unpacking keys:
 //
+//  * Bound by the reads: 256 sequences of 256 to 8192 tokens, 892.7 MB, in 154 us, 5.8 TB/s (the loads alone take 145); a
+//    single sequence by the latency of its few dependent loads and of the launch (7.2 us).
 //  * S^T = K Q^T by one v_mfma_scale_f32_16x16x128_f8f6f4 per 16 tokens: A is the record's 1 KiB of K codes as it
 //    lies in memory (16 bytes a lane) with the scale byte beside them, B is q in two 8-bit floats (split_query).
 //    hi of head c is column c and lo column c + 8 (a KV head has at most 8 query heads here); one row rotation adds
 //    the two products, and leaves every head twice, which does no harm.
 //  * C has the tokens in the A layout of P V's product (v_mfma_f32_16x16x32_bf16 over two records: lane quad r
-//    holds tokens 4 r .. 4 r + 3 of each), so the probabilities, rounded to bf16 (2^-9 of a weight, which the
-//    average of many takes further down, and half of what the output's own rounding costs), feed it without moving.
+//    holds tokens 4 r .. 4 r + 3 of each), so the probabilities, rounded to bf16 (half a step, 2^-8 of a weight at
+//    most, as the output's own rounding; the average over many tokens takes it further down), feed it without moving.
 //  * V: a lane loads the four tokens x eight dims that its part of B needs, two values a convert, and v_perm pairs
 //    the tokens.  Output tile t takes dim 8 j + t as its column j: a lane ends with eight dims of a head side by side.
 //  * The running maximum is raised only when a score passes it by 2^8 (with the sums scaled alike, exact).

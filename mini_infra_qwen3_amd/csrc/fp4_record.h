@@ -72,6 +72,12 @@ __device__ __forceinline__ int fp4_scale_at(bool value, int t, int j) {
 // that the instruction reads 8-bit operands in).  bf16 has 8 significant bits and e4m3 4, and the largest element's
 // hi is in [128, 256), so an element is exact down to 2^-14 of the largest, and off by at most 2^-23 of it below.
 // An infinity or NaN makes both scales NaN, and with them every score.
+//
+// The scaled product sums its 128 terms exactly down to about 2^-12 of the largest of them (measured: a term 2^-12.2 of
+// the largest is dropped), not to fp32.  That is a rounding of fewer bits than the kernels' other sums, and is taken because
+// the operands have less: q itself is bf16, off by up to 2^-9 of each term before it gets here, the largest one's error being
+// eight times what a term loses in the sum, and a key's code by up to a quarter of it.  lo's terms, 2^-4 of hi's, are
+// summed on their own and added in fp32.
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 struct SplitScale {
   float up;         // 2^-s: brings the largest element to [128, 256)
