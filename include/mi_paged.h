@@ -435,6 +435,19 @@ int32_t mi_qk_norm_rope(void* q_out, void* k_out, void* v_out, const void* q, in
                         int64_t num_slots, void* stream);
 
 /*
+ * mi_qk_norm_rope_fp4 -- mi_qk_norm_rope with slots in 4-bit pools: the k and v rows of a token with a slot are quantised into
+ * it as mi_reshape_and_cache_fp4 does, bit for bit; k_out / v_out (bf16) are optional.
+ * key_pool / value_pool: [num_slots / 16, Hkv, 1088] records, num_slots a multiple of 16; slot_mapping and the pools are
+ * required.  Rows, weights and pools must be 16-byte aligned, row strides multiples of 8.
+ */
+int32_t mi_qk_norm_rope_fp4(void* q_out, void* k_out, void* v_out, const void* q, int64_t q_stride, const void* k,
+                            int64_t k_stride, const void* v, int64_t v_stride, const void* q_weight,
+                            const void* k_weight, const void* cos, const void* sin, int64_t num_tokens,
+                            int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, float eps,
+                            const int64_t* slot_mapping, int64_t slot_stride, void* key_pool, void* value_pool,
+                            int64_t num_slots, void* stream);
+
+/*
  * mi_silu_mul -- the SwiGLU product of Qwen3MLP.forward (src/mini_infra/model/qwen3.py:347-355):
  *   out = bf16(bf16(silu(gate)) * up),  silu(g) = g / (1 + exp(-g)) in fp32.
  * gate / up / out: [rows, cols] with row element strides; cols and strides multiples of 8.

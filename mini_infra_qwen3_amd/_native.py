@@ -107,6 +107,11 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         [_ptr, _ptr, _ptr, _ptr, _i64, _ptr, _i64, _ptr, _i64, _ptr, _ptr, _ptr, _ptr, _i64, _i32, _i32, _i32,
          ctypes.c_float, _ptr, _i64, _ptr, _ptr, _i64, _ptr],
     ),
+    "mi_qk_norm_rope_fp4": (
+        _i32,
+        [_ptr, _ptr, _ptr, _ptr, _i64, _ptr, _i64, _ptr, _i64, _ptr, _ptr, _ptr, _ptr, _i64, _i32, _i32, _i32,
+         ctypes.c_float, _ptr, _i64, _ptr, _ptr, _i64, _ptr],
+    ),
     "mi_silu_mul": (_i32, [_ptr, _i64, _ptr, _i64, _ptr, _i64, _i64, _i32, _ptr]),
     "mi_argmax_rows": (_i32, [_ptr, _ptr, _i64, _i32, _i64, _ptr]),
     "mi_pack_blocks": (_i32, [_ptr, _c_void_p_p, _c_void_p_p, _i64, _ptr, _i64, _i32, _i64, _ptr]),

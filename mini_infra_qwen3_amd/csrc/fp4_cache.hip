@@ -4,9 +4,7 @@
 // reference's PagedKVCachePool.write_prefill, its decode append and PagedKVCachePool.gather_blocks
 // (src/mini_infra/worker/paged_kv_cache.py:54-95, src/mini_infra/model/qwen3.py:282-283).
 //
-// Both take a lane for eight values of a row (four code bytes), sixteen lanes for the row, so a group of 32 dims
-// is the four lanes of a DPP quad: its largest magnitude is two quad permutes away, in integer bits, which order
-// magnitudes and put every NaN above every number.
+// Both take a lane for eight values of a row (four code bytes), sixteen lanes for the row.
 #include "fp4_record.h"
 
 namespace mi {
@@ -107,20 +105,7 @@ __global__ __launch_bounds__(kThreads) void fp4_store_kernel(const StoreArgs a) 
   const int64_t record = (slot / kFp4Tokens) * a.kv_heads + h;
   const int t = static_cast<int>(slot % kFp4Tokens);
 #pragma unroll
-  for (int c = 0; c < 2; ++c) {
-    uint32_t amax = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) amax = max(amax, __float_as_uint(x[c][e]) & 0x7fffffffu);
-    amax = max(amax, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(amax), 0xB1, 0xf, 0xf, false)));
-    amax = max(amax, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(amax), 0x4E, 0xf, 0xf, false)));
-    const uint32_t scale = fp4_scale_code(amax);
-    const uint32_t codes = scale == kFp4NanScale ? 0u : fp4_pack8(x[c], e8m0_f32(scale));
-    if (live) {
-      char* p = a.pool[c][layer] + record * kFp4Record;
-      *reinterpret_cast<uint32_t*>(p + fp4_code_at(c == 1, t, j)) = codes;
-      if ((j & 3) == 0) *reinterpret_cast<uint8_t*>(p + fp4_scale_at(c == 1, t, j)) = static_cast<uint8_t>(scale);
-    }
-  }
+  for (int c = 0; c < 2; ++c) fp4_store_piece(a.pool[c][layer] + record * kFp4Record, c == 1, t, j, x[c], live);
 }
 
 struct GatherArgs {

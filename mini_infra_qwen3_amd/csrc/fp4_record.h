@@ -67,6 +67,23 @@ __device__ __forceinline__ int fp4_scale_at(bool value, int t, int j) {
   return kFp4Codes + (value ? 16 * (t >> 2) + 4 * (j >> 2) + (t & 3) : 16 * (j >> 2) + t);
 }
 
+// Quantises a row's piece j, dims 8 j .. 8 j + 7, into token t of a record.  Called by the sixteen lanes of a row together: a
+// group of 32 dims is the four lanes of a DPP quad, its largest magnitude two quad permutes away, in integer bits, which
+// order magnitudes and put every NaN above every number.
+__device__ __forceinline__ void fp4_store_piece(char* record, bool value, int t, int j, const float (&x)[8], bool live) {
+  uint32_t amax = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) amax = max(amax, __float_as_uint(x[e]) & 0x7fffffffu);
+  amax = max(amax, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(amax), 0xB1, 0xf, 0xf, false)));
+  amax = max(amax, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(amax), 0x4E, 0xf, 0xf, false)));
+  const uint32_t scale = fp4_scale_code(amax);
+  const uint32_t codes = scale == kFp4NanScale ? 0u : fp4_pack8(x, e8m0_f32(scale));
+  if (live) {
+    *reinterpret_cast<uint32_t*>(record + fp4_code_at(value, t, j)) = codes;
+    if ((j & 3) == 0) *reinterpret_cast<uint8_t*>(record + fp4_scale_at(value, t, j)) = static_cast<uint8_t>(scale);
+  }
+}
+
 // A query against K records: q = 2^s (hi + lo / 16), hi the nearest e4m3 numbers and lo the nearest ones of what is
 // left, as B operands of the scaled product (lane quad r holds dims 16 r .. + 15 and 64 + 16 r .. + 15, the order
 // that the instruction reads 8-bit operands in).  bf16 has 8 significant bits and e4m3 4, and the largest element's
@@ -75,8 +92,8 @@ __device__ __forceinline__ int fp4_scale_at(bool value, int t, int j) {
 //
 // The scaled product sums its 128 terms exactly down to about 2^-12 of the largest of them (measured: a term 2^-12.2 of
 // the largest is dropped), not to fp32.  That is a rounding of fewer bits than the kernels' other sums, and is taken because
-// the operands have less: q itself is bf16, off by up to 2^-9 of each term before it gets here, the largest one's error being
-// eight times what a term loses in the sum, and a key's code by up to a quarter of it.  lo's terms, 2^-4 of hi's, are
+// the operands have less: q itself is bf16, off by up to 2^-8 of each term before it gets here, the largest one's error being
+// sixteen times what a term loses in the sum, and a key's code by up to a quarter of it.  lo's terms, 2^-4 of hi's, are
 // summed on their own and added in fp32.
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 struct SplitScale {

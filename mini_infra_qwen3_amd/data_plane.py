@@ -751,7 +751,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_weight: to
     ``[num_blocks, block_size, Hkv, 128]`` at those slots (-1: skipped).  ``rows`` defaults to
     "no slot_mapping"; without rows ``(q_out, None, None)`` is returned (the decode form).
     ``k_out`` / ``v_out`` (optional): contiguous ``[T, Hkv, 128]`` buffers to write instead of new
-    ones.
+    ones.  4-bit pools (``fp4_pool_shape``) get the rows quantised, as ``reshape_and_cache_fp4`` writes them;
+    their rows must be 16-byte aligned.
     """
     device = q.device
     for name, t in (("q", q), ("k", k), ("v", v), ("q_weight", q_weight), ("k_weight", k_weight),
@@ -789,20 +790,30 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_weight: to
         _require_index("slot_mapping", slot_mapping, 1)
         if slot_mapping.shape[0] != tokens:
             raise ValueError(f"slot_mapping has {slot_mapping.shape[0]} entries for {tokens} tokens")
+        fp4 = key_pool is not None and key_pool.dtype is torch.uint8
         for name, pool in (("key_pool", key_pool), ("value_pool", value_pool)):
             if pool is None:
                 raise ValueError(f"{name} is required with slot_mapping")
+            if fp4:
+                continue
             _require_bf16_rows(name, pool, device)
             if not pool.is_contiguous() or pool.shape[-2:] != (num_kv_heads, head_dim):
                 raise ValueError(f"{name} must be contiguous [num_blocks, block_size, {num_kv_heads}, {head_dim}]")
-        num_slots = key_pool.numel() // (num_kv_heads * head_dim)
+        if fp4:
+            _require_gpu("key_pool", key_pool, device)
+            shape = _require_fp4_pools((key_pool,), (value_pool,)).shape
+            if shape[2] != num_kv_heads:
+                raise ValueError(f"4-bit pools have {shape[2]} KV heads, k has {num_kv_heads}")
+            num_slots = shape[0] * shape[1] * KERNEL_BLOCK_SIZE
+        else:
+            num_slots = key_pool.numel() // (num_kv_heads * head_dim)
         _check_range("slot_mapping", slot_mapping, num_slots, allow_minus_one=True)
-        rc = lib.mi_qk_norm_rope(q_out.data_ptr(), k_out.data_ptr() if rows else None,
-                                 v_out.data_ptr() if rows else None, q2.data_ptr(), q2.stride(0), k2.data_ptr(),
-                                 k2.stride(0), v2.data_ptr(), v2.stride(0), q_weight.data_ptr(), k_weight.data_ptr(),
-                                 cos2.data_ptr(), sin2.data_ptr(), tokens, num_heads, num_kv_heads, head_dim,
-                                 float(eps), slot_mapping.data_ptr(), slot_mapping.stride(0), key_pool.data_ptr(),
-                                 value_pool.data_ptr(), num_slots, _stream(device))
+        entry = lib.mi_qk_norm_rope_fp4 if fp4 else lib.mi_qk_norm_rope
+        rc = entry(q_out.data_ptr(), k_out.data_ptr() if rows else None, v_out.data_ptr() if rows else None,
+                   q2.data_ptr(), q2.stride(0), k2.data_ptr(), k2.stride(0), v2.data_ptr(), v2.stride(0),
+                   q_weight.data_ptr(), k_weight.data_ptr(), cos2.data_ptr(), sin2.data_ptr(), tokens, num_heads,
+                   num_kv_heads, head_dim, float(eps), slot_mapping.data_ptr(), slot_mapping.stride(0),
+                   key_pool.data_ptr(), value_pool.data_ptr(), num_slots, _stream(device))
     _native.check(rc, "mi_qk_norm_rope")
     return q_out, k_out, v_out
 

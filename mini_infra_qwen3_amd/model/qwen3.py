@@ -226,26 +226,23 @@ class Qwen3Attention(nn.Module):
         return self.o_proj(out), present
 
     def _fp4(self, q, k, v, cos, sin, kv_pool: PastKeyValue, metadata, workspace, kv_out=None):
-        """The three forms of ``forward`` on a 4-bit pool: q/k norm + RoPE, the store of the rows that have a slot, then
-        attention, a launch each (two more than the fused decode of 16-bit pools, whose append is part of the norm's).
-        A decoding token sees its own K/V as stored, in 4 bits; a chunk sees itself in bf16 and its history in 4 bits.
+        """The three forms of ``forward`` on a 4-bit pool: q/k norm + RoPE with the store of the rows that have a slot,
+        then attention.  A decoding token sees its own K/V as stored, in 4 bits; a chunk sees itself in bf16 and its
+        history in 4 bits.
 
-        A mixed step's chunk rows are laid out left-padded for the prefill kernel (one gather each of q, k and v, one
-        scatter of the output)."""
+        A mixed step stores its decode tokens in a launch of its own; its chunk rows are laid out left-padded for the
+        prefill kernel (one gather each of q, k and v, one scatter of the output)."""
         key_pool, value_pool = kv_pool
         heads, kv_heads, dim = self.num_heads, self.num_kv_heads, self.head_dim
         batch, length = q.shape[:2]
         k_buf, v_buf = kv_out if kv_out is not None else (None, None)
-        q_rot, k_rot, v_rows = data_plane.qk_norm_rope(q, k, v, self.q_norm.weight, self.k_norm.weight, cos, sin,
-                                                       self.q_norm.eps, k_out=k_buf, v_out=v_buf)
-
-        def store(first: int, slots):  # tokens [first, first + len(slots)), as rows of one token
-            n = slots.shape[0]
-            data_plane.reshape_and_cache_fp4([k_rot[first:first + n].unsqueeze(2)], [v_rows[first:first + n].unsqueeze(2)],
-                                             slots, [key_pool], [value_pool])
+        slots = None if isinstance(metadata, PagedMixedMetadata) else metadata.slot_mapping
+        q_rot, k_rot, v_rows = data_plane.qk_norm_rope(
+            q, k, v, self.q_norm.weight, self.k_norm.weight, cos, sin, self.q_norm.eps,
+            slot_mapping=None if slots is None else slots.reshape(-1), key_pool=key_pool, value_pool=value_pool,
+            k_out=k_buf, v_out=v_buf, rows=not isinstance(metadata, PagedAttentionMetadata))
 
         def decode(first: int, meta: PagedAttentionMetadata, out=None):
-            store(first, meta.slot_mapping)
             return data_plane.paged_decode_attention_fp4(
                 q_rot[first:first + meta.slot_mapping.shape[0]], key_pool, value_pool, meta.block_tables,
                 meta.context_lens, self.scaling, out=out, workspace=workspace)
@@ -258,13 +255,13 @@ class Qwen3Attention(nn.Module):
         if isinstance(metadata, PagedAttentionMetadata):
             return self.o_proj(decode(0, metadata).view(batch, 1, -1)), kv_pool
         if isinstance(metadata, PagedPrefillMetadata):
-            if metadata.slot_mapping is not None:
-                store(0, metadata.slot_mapping.reshape(-1))
             k_seq, v_seq = k_rot.view(batch, length, kv_heads, dim), v_rows.view(batch, length, kv_heads, dim)
             out = prefill(q_rot.view(batch, length, heads, dim), k_seq, v_seq, metadata)
             return self.o_proj(out), (k_seq.transpose(1, 2), v_seq.transpose(1, 2))
         rows, width, n = metadata.prefill_rows, metadata.prefill_width, metadata.chunk_span
         out = torch.zeros((length + 1, heads * dim), dtype=q_rot.dtype, device=q_rot.device)  # the last row: padding
+        data_plane.reshape_and_cache_fp4([k_rot[n:].unsqueeze(2)], [v_rows[n:].unsqueeze(2)], metadata.decode.slot_mapping,
+                                         [key_pool], [value_pool])
         decode(n, metadata.decode, out=out[n:length])
         if metadata.chunk_first is None:
             out[:n] = prefill(q_rot[:n].view(rows, width, heads, dim), k_rot[:n].view(rows, width, kv_heads, dim),

@@ -7,6 +7,21 @@ from mini_infra_qwen3_amd.model import PagedAttentionMetadata, Qwen3Config, Qwen
 from mini_infra_qwen3_amd.worker import KVBlockHeader, PagedKVCachePoolFp4
 
 
+@pytest.mark.skipif(torch.cuda.device_count() > 0, reason="host-only: placeholder pointers")
+def test_norm_rope_entry_refuses(native_lib):
+    good = dict(q_out=16, k_out=None, v_out=None, q=16, q_stride=2048, k=16, k_stride=1024, v=16, v_stride=1024, q_weight=16,
+                k_weight=16, cos=16, sin=16, tokens=3, heads=16, kv_heads=8, dim=128, eps=1e-6, slots=8, slot_stride=1,
+                key_pool=16, value_pool=16, num_slots=32, stream=None)
+    call = lambda **kw: native_lib.mi_qk_norm_rope_fp4(*{**good, **kw}.values())  # noqa: E731
+    assert call(tokens=0) == 0
+    for bad in (dict(tokens=-1), dict(heads=0), dict(kv_heads=0), dict(num_slots=-1), dict(dim=64), dict(q=None), dict(cos=None),
+                dict(slots=None), dict(key_pool=None), dict(value_pool=None), dict(k_out=16), dict(slot_stride=0),
+                dict(q_stride=2040), dict(k_stride=1016), dict(q=18), dict(v=8), dict(key_pool=8), dict(q_weight=4),
+                dict(k_out=8, v_out=16), dict(v_stride=1028), dict(tokens=1 << 40)):
+        assert call(**bad) != 0, bad
+        assert b"mi_qk_norm_rope_fp4" in native_lib.mi_last_error()
+
+
 def test_pool_needs_a_gpu():
     with pytest.raises(RuntimeError, match="GPU"):
         PagedKVCachePoolFp4(1, 4, 16, 8, 128, "cpu")

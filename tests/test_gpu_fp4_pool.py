@@ -240,6 +240,44 @@ def test_mixed_step_is_its_two_parts(native_lib, model, ragged, block_size):
         assert t.shape == shape and torch.equal(t.transpose(1, 2).reshape(c, 8, 128), flat[:c])
 
 
+@pytest.mark.parametrize("heads,kv_heads,block_size", [(16, 8, 16), (5, 1, 32), (6, 3, 48), (8, 8, 16)])
+@pytest.mark.parametrize("tokens", [1, 37])
+def test_norm_rope_stores_what_the_two_calls_store(native_lib, heads, kv_heads, block_size, tokens):
+    """Slots -1, past the pool and unwritten tokens' bytes included; a row with an infinity is stored as NaN."""
+    gen = torch.Generator().manual_seed(tokens + heads)
+    randn = lambda *shape: torch.randn(*shape, generator=gen).to(torch.bfloat16).cuda()  # noqa: E731
+    qkv = randn(tokens, (heads + 2 * kv_heads) * 128)
+    q, k, v = qkv[:, :heads * 128], qkv[:, heads * 128:(heads + kv_heads) * 128], qkv[:, (heads + kv_heads) * 128:]
+    if tokens > 1:
+        v[3, 40], k[4, 7] = float("inf"), float("nan")
+    weights, cos, sin = (1 + 0.1 * randn(128), 1 + 0.1 * randn(128)), randn(tokens, 128), randn(tokens, 128)
+    sub, blocks = block_size // 16, 4
+    slots = torch.randperm(blocks * block_size, generator=gen)[:tokens]
+    if tokens > 1:
+        slots[5], slots[9], slots[11] = -1, blocks * block_size, -7
+    table = torch.stack((slots, slots), 1).cuda()[:, 0]  # a stride of 2
+    rng = np.random.default_rng(tokens)
+    before = [fp4_ref.to_torch(fp4_ref.random_pool(rng, blocks * sub, kv_heads), sub).cuda() for _ in range(2)]
+    want = [p.clone() for p in before]
+    rows = data_plane.qk_norm_rope(q, k, v, *weights, cos, sin, 1e-6)
+    data_plane.reshape_and_cache_fp4([rows[1].unsqueeze(2)], [rows[2].unsqueeze(2)], table, [want[0]], [want[1]])
+    for keep in (True, False):
+        pools = [p.clone() for p in before]
+        got = data_plane.qk_norm_rope(q, k, v, *weights, cos, sin, 1e-6, slot_mapping=table, key_pool=pools[0],
+                                      value_pool=pools[1], rows=keep)
+        assert torch.equal(pools[0], want[0]) and torch.equal(pools[1], want[1])
+        for a, b in zip(got, rows if keep else (rows[0], None, None)):
+            assert a is b is None or torch.equal(a.view(torch.int16), b.view(torch.int16))
+    assert not torch.equal(want[0], before[0])
+    with pytest.raises(ValueError, match="KV heads"):
+        data_plane.qk_norm_rope(q, k, v, *weights, cos, sin, 1e-6, slot_mapping=table,
+                                key_pool=torch.zeros(2, 1, kv_heads + 1, 1088, dtype=torch.uint8, device="cuda"),
+                                value_pool=torch.zeros(2, 1, kv_heads + 1, 1088, dtype=torch.uint8, device="cuda"))
+    odd = torch.zeros(tokens, heads * 128 + 8, dtype=torch.bfloat16, device="cuda")[:, 1:heads * 128 + 1]
+    with pytest.raises(ValueError, match="aligned"):
+        data_plane.qk_norm_rope(odd, k, v, *weights, cos, sin, 1e-6, slot_mapping=table, key_pool=pools[0], value_pool=pools[1])
+
+
 def test_swap_and_files_keep_the_bytes(native_lib, tmp_path):
     pool = PagedKVCachePoolFp4(2, 12, 32, 3, 128, "cuda:0")
     gen = torch.Generator().manual_seed(0)
