@@ -616,15 +616,23 @@ enum class Form { kWide, kHalf, kHalfSplit, kNarrow, kSlim };
 // The workgroup shape of a launch, by the workgroups it would have in the narrow and the wide shape, and the parts of its keys.
 // Measured, us (16 query, 8 KV heads; rows x queries behind tokens of history, and the workgroups that decide),
 // wide / half / half split / narrow, and the keys cut into 4 / 8 / 16 parts:
-//   parts: twice the CUs' narrow workgroups, six tiles a part at least, three parts at least
+//   parts: twice the CUs' narrow workgroups, three parts at least, of six tiles at least, or twelve where the narrow
+//   workgroups alone keep more than 3/8 of the CUs busy (a second launch and its joining, and the partials, cost 8 us)
 //     1 x 1 behind 4000        8 narrow      138 / 105 /  76 /  53      27 / 20 / 18
 //     1 x 16 behind 20000      8             645 / 490 / 331 / 215      96 / 55 / 37
 //     1 x 60 behind 4000      16             140 / 110 /  79 /  52      29 / 24 / 23
 //     4 x 60 behind 2000      64              78 /  61 /  47 /  31      26 / 27 / 37
 //     1 x 300 behind 4000     80             148 / 116 /  84 /  57      40 / 42 / 49
+//     1 x 256 behind 1200     64                              23      21 (3 parts)
+//     1 x 333 behind 1500     88                              29      29 (4)
+//     2 x 256 behind 3000    128                              40      38 (4)
 //     1 x 512 behind 8000    128             219 / 153 / 123 /  88      63 / 68 / 81
 //   narrow: one round of its workgroups (cus; 11/8 of that without much history)
-//     2 x 333 behind 1500    176 narrow       68 /  53 /  41 /  29      35 / 39 / 56
+//     4 x 128 behind 1200    128 narrow                       23      28 (3 parts)
+//     3 x 160 behind 1500    120                              26      30 (4)
+//     2 x 256 behind 1500    128                              26      30 (4)
+//     5 x 100 behind 2000    160                              32      33 (3)
+//     2 x 333 behind 1500    176              68 /  53 /  41 /  29      35 / 39 / 56
 //     1 x 1000               256              41 /  34 /  26 /  19
 //   half: short rows without history
 //     15 x 128               120 wide         14 /  10 /  12 /  14
@@ -656,7 +664,8 @@ struct Plan {
     const int64_t wide = pairs * ((padded_len + Wide::kQTile - 1) / Wide::kQTile);
     const int64_t narrow = pairs * ((padded_len + Narrow::kQTile - 1) / Narrow::kQTile);
     const int64_t history = static_cast<int64_t>(max_history_blocks) * kFp4Tokens;
-    const int64_t most = std::min(2 * cus / narrow, (history + padded_len) / (6 * kKTile));
+    const int64_t part_tiles = 8 * narrow <= 3 * cus ? 6 : 12;
+    const int64_t most = std::min(2 * cus / narrow, (history + padded_len) / (part_tiles * kKTile));
     if (most >= 3) {
       form = Form::kSlim;
       parts = static_cast<int32_t>(most);
