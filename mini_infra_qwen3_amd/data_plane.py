@@ -808,7 +808,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_weight: to
         else:
             num_slots = key_pool.numel() // (num_kv_heads * head_dim)
         _check_range("slot_mapping", slot_mapping, num_slots, allow_minus_one=True)
-        entry = lib.mi_qk_norm_rope_fp4 if fp4 else lib.mi_qk_norm_rope
+        entry = lib.mi_qk_norm_rope if not fp4 else lambda *args: _on_device(device, "mi_qk_norm_rope_fp4", *args)
         rc = entry(q_out.data_ptr(), k_out.data_ptr() if rows else None, v_out.data_ptr() if rows else None,
                    q2.data_ptr(), q2.stride(0), k2.data_ptr(), k2.stride(0), v2.data_ptr(), v2.stride(0),
                    q_weight.data_ptr(), k_weight.data_ptr(), cos2.data_ptr(), sin2.data_ptr(), tokens, num_heads,
