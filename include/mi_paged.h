@@ -538,6 +538,11 @@ int32_t mi_copy_blocks(void* const* key_pools, void* const* value_pools, int64_t
  * (one that is not may also reach queries before it).  max_history_blocks is not limited by LDS.  workspace: at least
  * mi_chunked_prefill_fp4_workspace_bytes(...) bytes, as for decode: short chunks behind a long history have their keys cut over
  * workgroups, with partials there.
+ *
+ * mi_ragged_prefill_attention_fp4 -- the same for rows that lie back to back: query / key / value / out hold num_tokens tokens
+ * (head and token strides), row b the chunk_lens[b] ones from chunk_first[b * first_stride] on (clamped to [0, num_tokens -
+ * chunk_lens[b]]); max_len >= every chunk_lens (longer ones are cut to it, from their first token), and padded_len of the
+ * workspace's size.  Rows do not overlap; the output of tokens that no row covers is left as it was.
  */
 #define MI_TYPE_BF16 1
 #define MI_TYPE_FP16 2
@@ -572,6 +577,16 @@ int32_t mi_chunked_prefill_attention_fp4(void* out, int64_t out_row_stride, int6
                                          const int64_t* chunk_lens, int64_t lens_stride, int32_t batch,
                                          int32_t padded_len, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
                                          float scale, void* workspace, int64_t workspace_bytes, void* stream);
+int32_t mi_ragged_prefill_attention_fp4(void* out, int64_t out_tok_stride, const void* query, int64_t query_head_stride,
+                                        int64_t query_tok_stride, const void* key, int64_t key_head_stride,
+                                        int64_t key_tok_stride, const void* value, int64_t value_head_stride,
+                                        int64_t value_tok_stride, int32_t num_tokens, const void* key_pool,
+                                        const void* value_pool, int64_t num_blocks, const int64_t* history_blocks,
+                                        int64_t history_stride, int32_t max_history_blocks, const int64_t* start_lens,
+                                        const int64_t* chunk_lens, int64_t lens_stride, const int64_t* chunk_first,
+                                        int64_t first_stride, int32_t batch, int32_t max_len, int32_t num_heads,
+                                        int32_t num_kv_heads, int32_t head_dim, float scale, void* workspace,
+                                        int64_t workspace_bytes, void* stream);
 int64_t mi_chunked_prefill_fp4_workspace_bytes(int32_t batch, int32_t padded_len, int32_t num_heads,
                                                int32_t num_kv_heads, int32_t max_history_blocks);
 

@@ -137,6 +137,11 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         [_ptr, _i64, _i64, _ptr, _i64, _i64, _i64, _ptr, _i64, _i64, _i64, _ptr, _i64, _i64, _i64, _ptr, _ptr, _i64,
          _ptr, _i64, _i32, _ptr, _ptr, _i64, _i32, _i32, _i32, _i32, _i32, ctypes.c_float, _ptr, _i64, _ptr],
     ),
+    "mi_ragged_prefill_attention_fp4": (
+        _i32,
+        [_ptr, _i64, _ptr, _i64, _i64, _ptr, _i64, _i64, _ptr, _i64, _i64, _i32, _ptr, _ptr, _i64, _ptr, _i64, _i32, _ptr,
+         _ptr, _i64, _ptr, _i64, _i32, _i32, _i32, _i32, _i32, ctypes.c_float, _ptr, _i64, _ptr],
+    ),
     "mi_chunked_prefill_fp4_workspace_bytes": (_i64, [_i32, _i32, _i32, _i32, _i32]),
 }
 

@@ -86,6 +86,9 @@ struct Fp4PrefillArgs {
   const int64_t* start_lens;
   const int64_t* chunk_lens;
   int64_t lens_stride;
+  const int64_t* chunk_first;  // ragged rows: row b's first token among chunk_tokens, in row 0 of the tensors; null: padded rows
+  int64_t first_stride;
+  int32_t chunk_tokens;
   int32_t padded_len;
   int32_t kv_heads;
   int32_t group;  // query heads per KV head
@@ -98,6 +101,23 @@ struct Fp4PrefillArgs {
   float* ws_acc;  // [batch, heads, padded_len, parts, 128]
   float* ws_ml;   // [batch, heads, padded_len, parts, 2]: max (log2 units) and sum
   int32_t round_pairs;  // (row, head pair) units per dispatch round of one workgroup queue
+};
+
+// Where row b lies: its tokens, and what position i of its padded form has to move by to be token i + shift of row `row`.
+struct RowAt {
+  int len, row, shift;
+  __device__ __forceinline__ RowAt(const Fp4PrefillArgs& a, int b) {
+    const int64_t top = a.chunk_first ? min(a.padded_len, a.chunk_tokens) : a.padded_len;
+    const int64_t n = a.chunk_lens[b * a.lens_stride];
+    len = static_cast<int>(n < 0 ? 0 : (n > top ? top : n));
+    row = b;
+    shift = 0;
+    if (a.chunk_first) {
+      const int64_t first = a.chunk_first[b * a.first_stride], last = a.chunk_tokens - len;
+      row = 0;
+      shift = static_cast<int>(first < 0 ? 0 : (first > last ? last : first)) - (a.padded_len - len);
+    }
+  }
 };
 
 // A wavefront-uniform pointer that the compiler may hold in vector registers, in scalar ones.
@@ -141,10 +161,10 @@ __global__ __launch_bounds__(S::kThreads, 2) void fp4_prefill_kernel(const Fp4Pr
   }
   const int q0 = qt * kQTile;
   const int L = a.padded_len;
-  int64_t len64 = a.chunk_lens[b * a.lens_stride];
+  const RowAt place(a, b);
+  const int64_t src_row = __builtin_amdgcn_readfirstlane(place.row), shift = __builtin_amdgcn_readfirstlane(place.shift);
   int64_t start64 = a.start_lens[b * a.lens_stride];
-  len64 = len64 < 0 ? 0 : (len64 > L ? L : len64);
-  const int pad = __builtin_amdgcn_readfirstlane(L - static_cast<int>(len64));
+  const int pad = __builtin_amdgcn_readfirstlane(L - place.len);
   start64 = start64 < 0 ? 0 : start64;
   const int64_t hist_cap = static_cast<int64_t>(a.max_history_blocks) * kFp4Tokens;
   const int nh = __builtin_amdgcn_readfirstlane(static_cast<int>(start64 < hist_cap ? start64 : hist_cap));
@@ -164,9 +184,10 @@ __global__ __launch_bounds__(S::kThreads, 2) void fp4_prefill_kernel(const Fp4Pr
   const int ql = lane & 15;
   const int gq = lane >> 4;
 
-  uint16_t* out_b = a.out + b * a.out_row;
+  uint16_t* out_b = a.out + src_row * a.out_row + shift * a.out_tok;
+  if (pad == L && a.chunk_first) return;  // no tokens: nothing to read or write
   if (q0 + kQTile <= pad) {  // the whole tile is padding: zero rows
-    if (a.parts > 1) return;  // the second launch's
+    if (a.parts > 1 || a.chunk_first) return;  // the second launch's; or none
     for (int c = tid; c < kQTile * kGroup * (kHeadDim / 8); c += kThreads) {
       const int qi = q0 + c / (kGroup * (kHeadDim / 8));
       const int rem = c % (kGroup * (kHeadDim / 8));
@@ -178,7 +199,7 @@ __global__ __launch_bounds__(S::kThreads, 2) void fp4_prefill_kernel(const Fp4Pr
   }
 
   const int qw0 = q0 + kQPerWave * qs;  // first query of this wavefront
-  const uint16_t* q_rows = a.query + b * a.q_row + h * a.q_head;
+  const uint16_t* q_rows = a.query + src_row * a.q_row + shift * a.q_tok + h * a.q_head;
 
   // oacc[0..7]: O^T dims 16 dt + 4 gq + i of query column ql; oacc[8]: the weights' sums (its A operand has ones in
   // rows 0, 4, 8, 12).
@@ -429,8 +450,8 @@ __global__ __launch_bounds__(S::kThreads, 2) void fp4_prefill_kernel(const Fp4Pr
     }
     const int drow = lane >> 4;
     const int dchunk = lane & 15;
-    const uint16_t* k_rows = a.key + b * a.k_row + g * a.k_head;
-    const uint16_t* v_rows = a.value + b * a.v_row + g * a.v_head;
+    const uint16_t* k_rows = a.key + src_row * a.k_row + shift * a.k_tok + g * a.k_head;
+    const uint16_t* v_rows = a.value + src_row * a.v_row + shift * a.v_tok + g * a.v_head;
     const uint32_t k_tok = static_cast<uint32_t>(a.k_tok);  // < 2^24, checked by the entry point
     const uint32_t v_tok = static_cast<uint32_t>(a.v_tok);
     typedef __attribute__((address_space(3))) void* lds_ptr_t;
@@ -549,6 +570,7 @@ __global__ __launch_bounds__(S::kThreads, 2) void fp4_prefill_kernel(const Fp4Pr
     const int qi = qw0 + 16 * nt + ql;
     if (qi >= L || !head_live) continue;
     const bool real = qi >= pad;  // a padding row's sums are zeros, but a NaN among the values is in them too
+    if (!real && a.chunk_first) continue;
     const float inv = 1.0f / oacc[8][nt][0];
     uint16_t* orow = out_b + qi * a.out_tok + h * kHeadDim + 4 * gq;
 #pragma unroll
@@ -568,10 +590,10 @@ __global__ __launch_bounds__(kMergeThreads) void fp4_prefill_merge_kernel(const 
   if (row >= heads * a.padded_len * a.batch) return;
   const int64_t h = row % heads, qi = row / heads % a.padded_len, b = row / heads / a.padded_len;
   const int x = threadIdx.x & 31;
-  uint16_t* out = a.out + b * a.out_row + qi * a.out_tok + h * kHeadDim + 4 * x;
-  const int64_t len = a.chunk_lens[b * a.lens_stride];
-  if (qi < a.padded_len - len) {
-    *reinterpret_cast<uint2*>(out) = uint2{0u, 0u};
+  const RowAt place(a, static_cast<int>(b));
+  uint16_t* out = a.out + place.row * a.out_row + (qi + place.shift) * a.out_tok + h * kHeadDim + 4 * x;
+  if (qi < a.padded_len - place.len) {
+    if (!a.chunk_first) *reinterpret_cast<uint2*>(out) = uint2{0u, 0u};
     return;
   }
   const int64_t at = ((b * heads + h) * a.padded_len + qi) * a.parts;
@@ -685,29 +707,16 @@ struct Plan {
   int64_t bytes() const { return slots * (kHeadDim + 2) * static_cast<int64_t>(sizeof(float)); }
 };
 
-}  // namespace
-}  // namespace mi
-
-extern "C" int64_t mi_chunked_prefill_fp4_workspace_bytes(int32_t batch, int32_t padded_len, int32_t num_heads,
-                                                          int32_t num_kv_heads, int32_t max_history_blocks) {
-  using namespace mi;
-  if (batch <= 0 || padded_len <= 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0 ||
-      max_history_blocks < 0)
-    return 0;
-  return Plan(batch, padded_len, num_heads, num_kv_heads, max_history_blocks).bytes();
-}
-
-extern "C" int32_t mi_chunked_prefill_attention_fp4(
-    void* out, int64_t out_row_stride, int64_t out_tok_stride, const void* query, int64_t query_row_stride,
-    int64_t query_head_stride, int64_t query_tok_stride, const void* key, int64_t key_row_stride,
-    int64_t key_head_stride, int64_t key_tok_stride, const void* value, int64_t value_row_stride,
-    int64_t value_head_stride, int64_t value_tok_stride, const void* key_pool, const void* value_pool,
-    int64_t num_blocks, const int64_t* history_blocks, int64_t history_stride, int32_t max_history_blocks,
-    const int64_t* start_lens, const int64_t* chunk_lens, int64_t lens_stride, int32_t batch, int32_t padded_len,
-    int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, float scale, void* workspace, int64_t workspace_bytes,
-    void* stream) {
-  using namespace mi;
-  const char* name = "mi_chunked_prefill_attention_fp4";
+// The entry points below: chunk_first null for padded rows.
+int32_t run_prefill(const char* name, void* out, int64_t out_row_stride, int64_t out_tok_stride, const void* query,
+                    int64_t query_row_stride, int64_t query_head_stride, int64_t query_tok_stride, const void* key,
+                    int64_t key_row_stride, int64_t key_head_stride, int64_t key_tok_stride, const void* value,
+                    int64_t value_row_stride, int64_t value_head_stride, int64_t value_tok_stride, const void* key_pool,
+                    const void* value_pool, int64_t num_blocks, const int64_t* history_blocks, int64_t history_stride,
+                    int32_t max_history_blocks, const int64_t* start_lens, const int64_t* chunk_lens, int64_t lens_stride,
+                    const int64_t* chunk_first, int64_t first_stride, int32_t chunk_tokens, int32_t batch,
+                    int32_t padded_len, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, float scale,
+                    void* workspace, int64_t workspace_bytes, void* stream) {
   if (batch < 0 || padded_len < 0 || max_history_blocks < 0 || num_blocks < 0)
     return fail(MI_ERR_INVALID_ARGUMENT, "%s: negative size", name);
   if (batch == 0 || padded_len == 0) return ok();
@@ -761,6 +770,9 @@ extern "C" int32_t mi_chunked_prefill_attention_fp4(
   a.start_lens = start_lens;
   a.chunk_lens = chunk_lens;
   a.lens_stride = lens_stride;
+  a.chunk_first = chunk_first;
+  a.first_stride = first_stride;
+  a.chunk_tokens = chunk_tokens;
   a.padded_len = padded_len;
   a.kv_heads = num_kv_heads;
   a.group = num_heads / num_kv_heads;
@@ -789,4 +801,53 @@ extern "C" int32_t mi_chunked_prefill_attention_fp4(
     case Form::kNarrow: return launch<Narrow>(name, a, s);
     default: return launch<Slim>(name, a, s);
   }
+}
+
+}  // namespace
+}  // namespace mi
+
+extern "C" int64_t mi_chunked_prefill_fp4_workspace_bytes(int32_t batch, int32_t padded_len, int32_t num_heads,
+                                                          int32_t num_kv_heads, int32_t max_history_blocks) {
+  using namespace mi;
+  if (batch <= 0 || padded_len <= 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0 ||
+      max_history_blocks < 0)
+    return 0;
+  return Plan(batch, padded_len, num_heads, num_kv_heads, max_history_blocks).bytes();
+}
+
+extern "C" int32_t mi_chunked_prefill_attention_fp4(
+    void* out, int64_t out_row_stride, int64_t out_tok_stride, const void* query, int64_t query_row_stride,
+    int64_t query_head_stride, int64_t query_tok_stride, const void* key, int64_t key_row_stride,
+    int64_t key_head_stride, int64_t key_tok_stride, const void* value, int64_t value_row_stride,
+    int64_t value_head_stride, int64_t value_tok_stride, const void* key_pool, const void* value_pool,
+    int64_t num_blocks, const int64_t* history_blocks, int64_t history_stride, int32_t max_history_blocks,
+    const int64_t* start_lens, const int64_t* chunk_lens, int64_t lens_stride, int32_t batch, int32_t padded_len,
+    int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, float scale, void* workspace, int64_t workspace_bytes,
+    void* stream) {
+  return mi::run_prefill("mi_chunked_prefill_attention_fp4", out, out_row_stride, out_tok_stride, query, query_row_stride,
+                         query_head_stride, query_tok_stride, key, key_row_stride, key_head_stride, key_tok_stride, value,
+                         value_row_stride, value_head_stride, value_tok_stride, key_pool, value_pool, num_blocks,
+                         history_blocks, history_stride, max_history_blocks, start_lens, chunk_lens, lens_stride, nullptr, 0,
+                         0, batch, padded_len, num_heads, num_kv_heads, head_dim, scale, workspace, workspace_bytes, stream);
+}
+
+extern "C" int32_t mi_ragged_prefill_attention_fp4(
+    void* out, int64_t out_tok_stride, const void* query, int64_t query_head_stride, int64_t query_tok_stride,
+    const void* key, int64_t key_head_stride, int64_t key_tok_stride, const void* value, int64_t value_head_stride,
+    int64_t value_tok_stride, int32_t num_tokens, const void* key_pool, const void* value_pool, int64_t num_blocks,
+    const int64_t* history_blocks, int64_t history_stride, int32_t max_history_blocks, const int64_t* start_lens,
+    const int64_t* chunk_lens, int64_t lens_stride, const int64_t* chunk_first, int64_t first_stride, int32_t batch,
+    int32_t max_len, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, float scale, void* workspace,
+    int64_t workspace_bytes, void* stream) {
+  using namespace mi;
+  const char* name = "mi_ragged_prefill_attention_fp4";
+  if (num_tokens < 0) return fail(MI_ERR_INVALID_ARGUMENT, "%s: negative size", name);
+  if (batch > 0 && !chunk_first) return fail(MI_ERR_INVALID_ARGUMENT, "%s: null pointer argument", name);
+  if (first_stride <= 0) return fail(MI_ERR_INVALID_ARGUMENT, "%s: first_stride must be > 0", name);
+  if (num_tokens == 0) return ok();
+  return run_prefill(name, out, 0, out_tok_stride, query, 0, query_head_stride, query_tok_stride, key, 0, key_head_stride,
+                     key_tok_stride, value, 0, value_head_stride, value_tok_stride, key_pool, value_pool, num_blocks,
+                     history_blocks, history_stride, max_history_blocks, start_lens, chunk_lens, lens_stride, chunk_first,
+                     first_stride, num_tokens, batch, max_len, num_heads, num_kv_heads, head_dim, scale, workspace,
+                     workspace_bytes, stream);
 }

@@ -1227,6 +1227,8 @@ def chunked_prefill_attention_fp4(
     scale: float,
     out: torch.Tensor | None = None,
     workspace: torch.Tensor | None = None,
+    chunk_first: torch.Tensor | None = None,
+    max_len: int | None = None,
 ) -> torch.Tensor:
     """``chunked_prefill_attention`` with the history read from 4-bit pools (``fp4_pool_shape``).
 
@@ -1235,9 +1237,19 @@ def chunked_prefill_attention_fp4(
     Returns ``out`` ``[B, L, H * 128]`` bf16; left-padding rows are zero.  ``workspace`` (optional, uint8, reused
     across calls of one stream) holds the partials of short chunks behind long histories; it is allocated here when
     missing or too small.
+
+    Ragged rows: with ``chunk_first`` ``[B]`` int64 the tensors hold all rows' tokens back to back, ``[1, H, C, 128]``, and
+    row b is the ``chunk_lens[b]`` tokens from ``chunk_first[b]`` on, at most ``max_len``; rows do not overlap.  ``out``
+    ``[1, C, H * 128]`` then keeps what it held where no row is (zeros, if it is allocated here).
     """
     pool0 = _require_fp4_pools((key_pool,), (value_pool,))
     device, index = pool0.device, pool0.get_device()
+    ragged = chunk_first is not None
+    if ragged:
+        if max_len is None or max_len < 0:
+            raise ValueError("chunk_first needs max_len >= 0")
+        _require_gpu("chunk_first", chunk_first, device)
+        _require_index("chunk_first", chunk_first, 1)
     for name, t in (("query", query), ("key", key), ("value", value), ("history_blocks", history_blocks),
                     ("start_lens", start_lens), ("chunk_lens", chunk_lens)):
         if t.get_device() != index:
@@ -1252,15 +1264,22 @@ def chunked_prefill_attention_fp4(
     num_blocks, sub, num_kv_heads, _ = pool0.shape
     if key.shape != (batch, num_kv_heads, padded_len, head_dim) or value.shape != key.shape:
         raise ValueError(f"key/value must be [{batch}, {num_kv_heads}, {padded_len}, {head_dim}]")
+    tensor_rows = batch
+    if ragged:
+        if batch != 1:
+            raise ValueError(f"with chunk_first the tensors hold one row of tokens, got {batch}")
+        batch = chunk_first.shape[0]
     if history_blocks.shape[0] != batch or start_lens.shape[0] != batch or chunk_lens.shape[0] != batch:
         raise ValueError("history_blocks / start_lens / chunk_lens batch differs from query batch")
     if out is None:
-        out = torch.empty((batch, padded_len, num_heads * head_dim), dtype=torch.bfloat16, device=device)
+        shape = (tensor_rows, padded_len, num_heads * head_dim)
+        out = (torch.zeros if ragged else torch.empty)(shape, dtype=torch.bfloat16, device=device)
     else:
         _require_gpu("out", out, device)
-        if out.shape != (batch, padded_len, num_heads * head_dim) or out.dtype is not torch.bfloat16 or out.stride(2) != 1:
+        if out.shape != (tensor_rows, padded_len, num_heads * head_dim) or out.dtype is not torch.bfloat16 or out.stride(2) != 1:
             raise ValueError(f"out must be [B, L, H * D] bf16 with unit inner stride, got {tuple(out.shape)}")
-    if batch == 0 or padded_len == 0:
+    width = max_len if ragged else padded_len
+    if batch == 0 or padded_len == 0 or width == 0:
         return out
     _check_range("history_blocks", history_blocks, num_blocks)
     if sub > 1:
@@ -1270,16 +1289,25 @@ def chunked_prefill_attention_fp4(
         history_blocks = history_blocks.contiguous()
     if batch > 1 and (start_lens.stride(0) != chunk_lens.stride(0) or start_lens.stride(0) <= 0):
         start_lens, chunk_lens = start_lens.contiguous(), chunk_lens.contiguous()
-    need = _on_device(device, "mi_chunked_prefill_fp4_workspace_bytes", batch, padded_len, num_heads, num_kv_heads, nb)
+    need = _on_device(device, "mi_chunked_prefill_fp4_workspace_bytes", batch, width, num_heads, num_kv_heads, nb)
     ws_ptr, ws_bytes, workspace = _workspace(workspace, need, device)
 
     def strides(t):  # of a dim of one element any stride is good
         return [st if n > 1 else 0 for st, n in zip(t.stride()[:-1], t.shape)]
 
+    history = (history_blocks.data_ptr() if nb else None, (history_blocks.stride(0) if batch > 1 else nb) if nb else 0, nb)
+    lens = (start_lens.data_ptr(), chunk_lens.data_ptr(), start_lens.stride(0) if batch > 1 else 1)
+    if ragged:
+        if batch > 1 and chunk_first.stride(0) <= 0:
+            chunk_first = chunk_first.contiguous()
+        _call(device, "mi_ragged_prefill_attention_fp4", out.data_ptr(), *strides(out)[1:], query.data_ptr(),
+              *strides(query)[1:], key.data_ptr(), *strides(key)[1:], value.data_ptr(), *strides(value)[1:], padded_len,
+              key_pool.data_ptr(), value_pool.data_ptr(), num_blocks, *history, *lens, chunk_first.data_ptr(),
+              chunk_first.stride(0) if batch > 1 else 1, batch, width, num_heads, num_kv_heads, head_dim, float(scale),
+              ws_ptr, ws_bytes, _stream(device))
+        return out
     _call(device, "mi_chunked_prefill_attention_fp4", out.data_ptr(), *strides(out), query.data_ptr(), *strides(query),
           key.data_ptr(), *strides(key), value.data_ptr(), *strides(value),
-          key_pool.data_ptr(), value_pool.data_ptr(), num_blocks, history_blocks.data_ptr() if nb else None,
-          (history_blocks.stride(0) if batch > 1 else nb) if nb else 0, nb, start_lens.data_ptr(), chunk_lens.data_ptr(),
-          start_lens.stride(0) if batch > 1 else 1, batch, padded_len, num_heads, num_kv_heads, head_dim, float(scale),
+          key_pool.data_ptr(), value_pool.data_ptr(), num_blocks, *history, *lens, batch, padded_len, num_heads, num_kv_heads, head_dim, float(scale),
           ws_ptr, ws_bytes, _stream(device))
     return out

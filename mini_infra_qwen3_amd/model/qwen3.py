@@ -230,8 +230,7 @@ class Qwen3Attention(nn.Module):
         then attention.  A decoding token sees its own K/V as stored, in 4 bits; a chunk sees itself in bf16 and its
         history in 4 bits.
 
-        A mixed step stores its decode tokens in a launch of its own; its chunk rows are laid out left-padded for the
-        prefill kernel (one gather each of q, k and v, one scatter of the output)."""
+        A mixed step stores its decode tokens in a launch of their own and runs both attentions."""
         key_pool, value_pool = kv_pool
         heads, kv_heads, dim = self.num_heads, self.num_kv_heads, self.head_dim
         batch, length = q.shape[:2]
@@ -247,10 +246,10 @@ class Qwen3Attention(nn.Module):
                 q_rot[first:first + meta.slot_mapping.shape[0]], key_pool, value_pool, meta.block_tables,
                 meta.context_lens, self.scaling, out=out, workspace=workspace)
 
-        def prefill(q_rows, k_rows, v_rows, meta: PagedPrefillMetadata):  # [B, L, H, D] each
+        def prefill(q_rows, k_rows, v_rows, meta: PagedPrefillMetadata, **kw):  # [B, L, H, D] each
             return data_plane.chunked_prefill_attention_fp4(
                 q_rows.transpose(1, 2), k_rows.transpose(1, 2), v_rows.transpose(1, 2), key_pool, value_pool,
-                meta.history_block_tables, meta.start_lens, meta.chunk_lens, self.scaling, workspace=workspace)
+                meta.history_block_tables, meta.start_lens, meta.chunk_lens, self.scaling, workspace=workspace, **kw)
 
         if isinstance(metadata, PagedAttentionMetadata):
             return self.o_proj(decode(0, metadata).view(batch, 1, -1)), kv_pool
@@ -259,25 +258,16 @@ class Qwen3Attention(nn.Module):
             out = prefill(q_rot.view(batch, length, heads, dim), k_seq, v_seq, metadata)
             return self.o_proj(out), (k_seq.transpose(1, 2), v_seq.transpose(1, 2))
         rows, width, n = metadata.prefill_rows, metadata.prefill_width, metadata.chunk_span
-        out = torch.zeros((length + 1, heads * dim), dtype=q_rot.dtype, device=q_rot.device)  # the last row: padding
+        out = torch.zeros((length, heads * dim), dtype=q_rot.dtype, device=q_rot.device)  # tokens of no row stay zeros
         data_plane.reshape_and_cache_fp4([k_rot[n:].unsqueeze(2)], [v_rows[n:].unsqueeze(2)], metadata.decode.slot_mapping,
                                          [key_pool], [value_pool])
         decode(n, metadata.decode, out=out[n:length])
-        if metadata.chunk_first is None:
-            out[:n] = prefill(q_rot[:n].view(rows, width, heads, dim), k_rot[:n].view(rows, width, kv_heads, dim),
-                              v_rows[:n].view(rows, width, kv_heads, dim), metadata.prefill).view(n, -1)
-            per_row = (rows, width)
-        else:
-            lens = metadata.prefill.chunk_lens.clamp(0, min(width, n)).unsqueeze(1)
-            first = torch.minimum(metadata.chunk_first.unsqueeze(1).clamp(min=0), n - lens)
-            ahead = torch.arange(width, device=q_rot.device) - (width - lens)  # token of the row, negative in its padding
-            token = torch.where(ahead >= 0, first + ahead, 0).reshape(-1)
-            chunk = [t.index_select(0, token).view(rows, width, *t.shape[1:]) for t in (q_rot, k_rot, v_rows)]
-            padded = prefill(*chunk, metadata.prefill).view(rows * width, -1)
-            out.index_copy_(0, torch.where(ahead.reshape(-1) >= 0, token, length), padded)
-            per_row = (1, n)
+        per_row = (rows, width) if metadata.chunk_first is None else (1, n)
+        chunk = [t[:n].view(*per_row, *t.shape[1:]) for t in (q_rot, k_rot, v_rows)]
+        ragged = {} if metadata.chunk_first is None else {"chunk_first": metadata.chunk_first, "max_len": width}
+        prefill(*chunk, metadata.prefill, out=out[:n].view(*per_row, -1), **ragged)
         present = tuple(t[:n].view(*per_row, kv_heads, dim).transpose(1, 2) for t in (k_rot, v_rows))
-        return self.o_proj(out[:length].unsqueeze(0)), present
+        return self.o_proj(out.unsqueeze(0)), present
 
     def _mixed(self, q, k, v, cos, sin, kv_pool: PastKeyValue, metadata: PagedMixedMetadata, workspace, kv_out=None):
         """One q/k norm + RoPE launch over all T tokens, then one attention launch for the chunk rows
