@@ -114,6 +114,12 @@ class PagedMixedMetadata(NamedTuple):
         return self.chunk_tokens if self.chunk_first is not None else self.prefill_rows * self.prefill_width
 
 
+def mixed_slots(metadata: PagedMixedMetadata) -> torch.Tensor:
+    """``[T]`` int64: the pool slots of a mixed step's decode tokens, -1 for its chunk tokens (stored later)."""
+    slots = metadata.decode.slot_mapping
+    return torch.cat((slots.new_full((metadata.chunk_span,), -1), slots))
+
+
 class RMSNorm(nn.Module):
     """RMSNorm weight holder (reference qwen3.py:55-78).  The norm itself runs fused with the
     preceding residual add in ``data_plane.rms_norm`` (fp32 inside, reference rounding points)."""
@@ -230,12 +236,16 @@ class Qwen3Attention(nn.Module):
         then attention.  A decoding token sees its own K/V as stored, in 4 bits; a chunk sees itself in bf16 and its
         history in 4 bits.
 
-        A mixed step stores its decode tokens in a launch of their own and runs both attentions."""
+        A mixed step runs both attentions; its slots are -1 for the chunk tokens (``mixed_slots``, built once a step)."""
         key_pool, value_pool = kv_pool
         heads, kv_heads, dim = self.num_heads, self.num_kv_heads, self.head_dim
         batch, length = q.shape[:2]
         k_buf, v_buf = kv_out if kv_out is not None else (None, None)
-        slots = None if isinstance(metadata, PagedMixedMetadata) else metadata.slot_mapping
+        if isinstance(metadata, PagedMixedMetadata):
+            slots = metadata.prefill.slot_mapping
+            slots = mixed_slots(metadata) if slots is None else slots
+        else:
+            slots = metadata.slot_mapping
         q_rot, k_rot, v_rows = data_plane.qk_norm_rope(
             q, k, v, self.q_norm.weight, self.k_norm.weight, cos, sin, self.q_norm.eps,
             slot_mapping=None if slots is None else slots.reshape(-1), key_pool=key_pool, value_pool=value_pool,
@@ -259,8 +269,6 @@ class Qwen3Attention(nn.Module):
             return self.o_proj(out), (k_seq.transpose(1, 2), v_seq.transpose(1, 2))
         rows, width, n = metadata.prefill_rows, metadata.prefill_width, metadata.chunk_span
         out = torch.zeros((length, heads * dim), dtype=q_rot.dtype, device=q_rot.device)  # tokens of no row stay zeros
-        data_plane.reshape_and_cache_fp4([k_rot[n:].unsqueeze(2)], [v_rows[n:].unsqueeze(2)], metadata.decode.slot_mapping,
-                                         [key_pool], [value_pool])
         decode(n, metadata.decode, out=out[n:length])
         per_row = (rows, width) if metadata.chunk_first is None else (1, n)
         chunk = [t[:n].view(*per_row, *t.shape[1:]) for t in (q_rot, k_rot, v_rows)]
@@ -389,6 +397,7 @@ class Qwen3Model(nn.Module):
             if len(pools) != len(self.layers):
                 raise ValueError("kv_pools has a different number of layers than the model")
             if self._fp4_pools(pools):
+                metadata = metadata._replace(prefill=metadata.prefill._replace(slot_mapping=mixed_slots(metadata)))
                 need = max(self._fp4_decode_bytes(decode_rows, metadata.decode.block_tables, pools),
                            self._fp4_prefill_bytes(rows, metadata.prefill_width, metadata.prefill.history_block_tables, pools))
             else:
