@@ -7,8 +7,9 @@
 //
 // Like the block records (kv_block_records.hip), kSplit workgroups share one layer's K or V block, 16 bytes a lane, but
 // a layer's K or V is done for all pairs before the next: 1000 blocks of 28 layers of a 2200-block pool (1.84 GB each way)
-// 666 us, 5.5 TB/s; with all layers of a pair in turn, as records lie, 728.  Splits of 8 and 16, other stores and runs per
-// XCD within 1%; one workgroup a block 693.
+// 666 us, 5.5 TB/s; with all layers of a pair in turn, as records lie, 728.  Splits of 8 to 32 with
+// fewer threads, other stores and runs per XCD within 1%; one workgroup a block 693, ordinary loads 684, 512 or 1024 threads
+// 685 to 704.  (Copies into randomly placed 32 KiB units reach 5.6 to 5.7 TB/s on this card.)
 #include "mi_common.h"
 
 namespace mi {
