@@ -281,10 +281,15 @@ __global__ __launch_bounds__(64 * kWaves, kPartWavesPerSimd) void fp4_part_kerne
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
   const int j = lane & 15, r = lane >> 4;
+  const int first = part * a.part_blocks;  // < max_blocks, but for an empty table
+  // Lanes 2 k and 2 k + 1 hold the ids of the wavefront's k-th pair, blocks 2 w + 2 k kWaves and the next.  They are read
+  // before the context's length is known, a memory round trip earlier; what lies past it is not used.
+  const int mine = 2 * w + kWaves * (lane & ~1) + (lane & 1);
+  int64_t id = 0;
+  if (a.max_blocks > 0) id = a.block_tables[b * a.bt_stride + min(first + mine, a.max_blocks - 1)];
   const int64_t n = tokens_of(a, b);
   uint16_t* out = a.out + b * a.out_row + static_cast<int64_t>(g) * a.group * kHeadDim;
   const int blocks = blocks_of(n);
-  const int first = part * a.part_blocks;  // < max_blocks
   if (first >= blocks) {                   // uniform
     if (part == 0)                         // an empty context: zero rows
       for (int c = threadIdx.x; c < a.group * 16; c += kThreads) *reinterpret_cast<u32x4*>(out + 8 * c) = u32x4{};
@@ -292,8 +297,7 @@ __global__ __launch_bounds__(64 * kWaves, kPartWavesPerSimd) void fp4_part_kerne
   }
   const int count = min(a.part_blocks, blocks - first);
   Walk walk(a, g, lane);
-  // Lanes 2 k and 2 k + 1 hold the ids of the wavefront's k-th pair, blocks 2 w + 2 k kWaves and the next.
-  walk.ids = Walk::fetch_id(a, a.block_tables + b * a.bt_stride + first, count, 2 * w + kWaves * (lane & ~1) + (lane & 1));
+  walk.ids = mine < count && id >= 0 && id < a.num_blocks ? static_cast<uint32_t>(id) : 0u;  // the null block, hidden there
   MfmaState st;
   start(st);
   // The context's end as the part sees it: a pair past the part's own blocks is hidden.
