@@ -6,7 +6,7 @@
 // reference's gather, mask and attend: src/mini_infra/model/qwen3.py:219-292) for 136 bytes a token and KV head
 // instead of 512.  At that size a bf16 kernel's arithmetic would be the bound, so none is spent on unpacking keys:
 //
-//  * Bound by the reads: 256 sequences of 256 to 8192 tokens, 892.7 MB, in 154 us, 5.8 TB/s (the loads alone take 145); a
+//  * Bound by the reads: 256 sequences of 256 to 8192 tokens, 892.7 MB, in 151 us, 5.9 TB/s (the loads alone take 145); a
 //    single sequence by the latency of its few dependent loads and of the launch (7.2 us).
 //  * S^T = K Q^T by one v_mfma_scale_f32_16x16x128_f8f6f4 per 16 tokens: A is the record's 1 KiB of K codes as it
 //    lies in memory (16 bytes a lane) with the scale byte beside them, B is q in two 8-bit floats (split_query).
@@ -303,10 +303,8 @@ __global__ __launch_bounds__(64 * kWaves, kPartWavesPerSimd) void fp4_part_kerne
   // The context's end as the part sees it: a pair past the part's own blocks is hidden.
   const int64_t end = min(n - static_cast<int64_t>(first) * kFp4Tokens, static_cast<int64_t>(count) * kFp4Tokens);
   int i = 2 * w;
-  if (i < count) {
-    walk.load_k(0);
-    walk.load_v(0);
-  }
+  walk.load_k(0);
+  walk.load_v(0);
   stage_queries(s_q, a, b, g);
   __syncthreads();
   i32x8 q;
@@ -320,12 +318,12 @@ __global__ __launch_bounds__(64 * kWaves, kPartWavesPerSimd) void fp4_part_kerne
     }
   }
   const uint32_t q_scale = s_q.scales[j >> 3][j & 7];
+  // Loads without a condition, of the null block after the last pair: the waits then cover a pair's own loads only (64
+  // sequences 14.4 us instead of 15.2, 21 of 64 heads 26.3 instead of 27.5).
   for (int k = 2; i < count; i += 2 * kWaves, k += 2) {
-    const bool more = i + 2 * kWaves < count;
-    walk.attend(st, q, q_scale, a.scale, end - static_cast<int64_t>(i) * kFp4Tokens, r, [&] {
-      if (more) walk.load_k(k);
-    });
-    if (more) walk.load_v(k);
+    const int ahead = min(k, kIds - 2);
+    walk.attend(st, q, q_scale, a.scale, end - static_cast<int64_t>(i) * kFp4Tokens, r, [&] { walk.load_k(ahead); });
+    walk.load_v(ahead);
   }
   const float l = xsum32_f32(xsum16_f32(st.l));  // lane: head lane % 8
 #pragma unroll
@@ -468,10 +466,10 @@ __global__ __launch_bounds__(64 * kStreamWaves, kStreamWavesPerSimd) void fp4_st
     const int64_t visible = min(tokens_of(a, seg.b) - static_cast<int64_t>(seg.first) * kFp4Tokens, static_cast<int64_t>(count) * kFp4Tokens);
     MfmaState st;
     start(st);
-    for (int i = 0, ahead = 2; i < count; i += 2, ahead += 2) {  // ahead: the next pair's place in the window of ids
-      bool more = true;
+    // ahead: the next pair's place in the window of ids.  After the range's last pair the null block is loaded (see the
+    // parts form; 154 us to 151 at 256 sequences).
+    for (int i = 0, ahead = 2; i < count; i += 2, ahead += 2) {
       if (i + 2 >= count) {
-        more = another;
         ahead = 0;
         walk.ids = ids_ahead;
       } else if (ahead == kIds) {
@@ -479,10 +477,8 @@ __global__ __launch_bounds__(64 * kStreamWaves, kStreamWavesPerSimd) void fp4_st
         walk.ids = ids_next;
         if (count - i - 2 > kIds) ids_next = Walk::fetch_id(a, row + i + 2 + kIds, count - i - 2 - kIds, lane);
       }
-      walk.attend(st, q, q_scale, a.scale, visible - static_cast<int64_t>(i) * kFp4Tokens, r, [&] {
-        if (more) walk.load_k(ahead);
-      });
-      if (more) walk.load_v(ahead);
+      walk.attend(st, q, q_scale, a.scale, visible - static_cast<int64_t>(i) * kFp4Tokens, r, [&] { walk.load_k(ahead); });
+      walk.load_v(ahead);
     }
     const float l = xsum32_f32(xsum16_f32(st.l));
     uint16_t* out = a.out + seg.b * a.out_row + static_cast<int64_t>(g) * a.group * kHeadDim + 8 * j;
