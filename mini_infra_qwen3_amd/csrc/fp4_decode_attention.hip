@@ -25,6 +25,8 @@
 //  * Streams: the blocks of all sequences, in order, are cut into as many equal ranges as the device holds wavefronts
 //    (per KV head), whatever the lengths; a wavefront walks its range, sequence by sequence.  Sequences that
 //    a range's end cuts leave partials, two a range at most, for the second launch.
+#include <algorithm>
+
 #include "decode_block.h"
 #include "fp4_record.h"
 
@@ -570,23 +572,26 @@ __global__ __launch_bounds__(kMergeThreads) void fp4_merge_kernel(const Fp4Decod
 // How a launch is cut, and the workspace that takes, by the (sequence, KV head) pairs P, the table's blocks M and their
 // product (context lengths are on the device).  Measured, us a call (16 query / 8 KV heads but where noted; lengths in
 // tokens, M their longest's blocks), whole sequences by 4 / by 8 wavefronts, parts of 16 / 32 / 64 blocks, streams:
-//   whole, 8 wavefronts to 2 P a CU, then 4: a second launch and its joining cost 4 to 5 us, more than short tables' tail
-//       1 x 417             M 27    P 8      6.7 /  6.9     8.4 /   6.6 /   6.7    10.4
-//       8 x 32..1150           72      64   10.7 /  9.4    10.2 /  11.2 /  14.0    14.5
-//      64 x 32..1150           72     512   16.2 / 14.2    20.4 /  19.5 /  22.5    21.6
-//     128 x 32..1150           72    1024   21.9 / 24.8    31.2 /  27.6 /  36.4    29.1
-//    1000 x 32..1150           72    8000    124 /  154     187 /   163 /   206     144
-//      64 x 50..3500          219     512   38.4 / 30.9    39.3 /  32.8 /  42.1    33.4
+//   whole, 8 wavefronts to 2 P a CU, then 4: a second launch and its joining cost 4 to 5 us, more than the tail of tables of
+//   80 blocks, or of 256 where P fills the CUs, and in proportion between
+//       1 x 417             M 27    P 8      6.5 /  6.9     8.4 /   6.5 /   6.5    10.2
+//       8 x 32..1150           72      64   10.1 /  8.9    10.0 /  10.0 /  11.8    14.3
+//      16 x 1000..2000        125     128   16.2 / 12.5    13.6 /  13.0 /  14.4    18.3
+//      20 x 1200..2550        160     160      - / 16.1    15.7 (by rule)
+//      31 x 2000..3900        244     248      - / 24.0    27.4 (by rule)
+//      64 x 32..1150           72     512   15.4 / 14.7    21.4 /  19.6 /  22.2    22.5
+//     128 x 32..1150           72    1024   21.9 / 24.5    32.0 /  27.6 /  35.2    30.2
+//    1000 x 32..1150           72    8000    121 /  151     189 /   165 /   201     144
+//      64 x 50..3500          219     512   31.9 / 31.1    39.8 /  32.9 /  41.1    34.4
 //   parts: few pairs
-//       1 x 4000              250       8   17.1 / 19.0     8.8 /   9.7 /  12.1    11.6
-//      16 x 1000..2000        125     128   19.2 / 13.8    13.5 /  13.5 /  15.6    17.9
-//       1 x 65000            4063       8           -      31.3 /  22.9 /  22.6    35.7
-//       4 x 20000..40000     2500      32           -      40.0 /  32.0 /  29.8    35.2
-//      21 x 256..8192, 64 query heads  512  168     -      30.2 /  25.9 /  26.5    29.1
+//       1 x 4000              250       8   26.1 / 18.6     9.5 /  10.6 /  13.2    13.0
+//       1 x 65000            4063       8           -      31.6 /  23.8 /  21.6    37.1
+//       4 x 20000..40000     2500      32           -      40.5 /  33.1 /  30.8    35.9
+//      21 x 256..8192, 64 query heads  512  168     - / 35.3   31.5 /  26.1 /  26.2    29.9
 //   streams: long tables of many pairs, mostly empty
-//      30 x 256..8192         512     240           -      35.0 /  30.9 /  32.5    29.9
-//     100 x 256..8192         512     800           -      90.4 /  79.6 /  80.3    65.6
-//     256 x 256..8192         512    2048           -         - /     - /   254     154
+//      30 x 256..8192         512     240      - / 36.9    37.1 /  31.6 /  32.1    31.3
+//     100 x 256..8192         512     800      - / 73.4    93.9 /  79.9 /  78.4    63.3
+//     256 x 256..8192         512    2048      -  / 170     241 /   209 /   199     152
 struct Plan {
   int32_t streams, part_blocks, parts, waves;
   int64_t slots, bytes;
@@ -599,7 +604,8 @@ struct Plan {
     waves = pairs <= 2 * cus ? 8 : 4;
     part_blocks = max_blocks > 0 ? max_blocks : 1;
     slots = bytes = 0;
-    if (max_blocks <= (pairs >= cus ? 4 * kIds : 80)) return;  // whole: every wavefront's ids fit its lanes
+    // whole: every wavefront's ids fit its lanes
+    if (max_blocks <= std::min<int64_t>(std::max<int64_t>(pairs * 4 * kIds / cus, 80), 4 * kIds)) return;
     waves = 4;
     if (batch <= kMaxStreamBatch && units >= 120000 && static_cast<int64_t>(batch) * max_blocks < (int64_t{1} << 30)) {
       const int64_t s = cus * 4 * kStreamWavesPerSimd / num_kv_heads;
