@@ -7,7 +7,7 @@
 // instead of 512.  At that size a bf16 kernel's arithmetic would be the bound, so none is spent on unpacking keys:
 //
 //  * Bound by the reads: 256 sequences of 256 to 8192 tokens, 892.7 MB, in 151 us, 5.9 TB/s (the loads alone take 145); a
-//    single sequence by the latency of its few dependent loads and of the launch (7.2 us).
+//    single sequence by the latency of its few dependent loads and of the launch (6.9 us).
 //  * S^T = K Q^T by one v_mfma_scale_f32_16x16x128_f8f6f4 per 16 tokens: A is the record's 1 KiB of K codes as it
 //    lies in memory (16 bytes a lane) with the scale byte beside them, B is q in two 8-bit floats (split_query).
 //    hi of head c is column c and lo column c + 8 (a KV head has at most 8 query heads here); one row rotation adds
@@ -331,39 +331,36 @@ __global__ __launch_bounds__(64 * kWaves, kPartWavesPerSimd) void fp4_part_kerne
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int h = 4 * r + i;
-    const float lh = __shfl(l, h & 7), mh = __shfl(st.m, h & 7);
     if (h >= a.group) continue;
     float4* dst = reinterpret_cast<float4*>(s_raw + (w * a.group + h) * kHeadDim + 8 * j);
     dst[0] = make_float4(st.o[0][i], st.o[1][i], st.o[2][i], st.o[3][i]);
     dst[1] = make_float4(st.o[4][i], st.o[5][i], st.o[6][i], st.o[7][i]);
-    if (j == 0) *reinterpret_cast<float2*>(s_ml + (w * a.group + h) * 2) = make_float2(mh, lh);
   }
+  if (lane < a.group) *reinterpret_cast<float2*>(s_ml + (w * a.group + lane) * 2) = make_float2(st.m, l);
   __syncthreads();
   const bool whole = blocks <= a.part_blocks;
-  for (int x8 = threadIdx.x; x8 < a.group * 16; x8 += kThreads) {
-    const int h = x8 >> 4, o8 = 8 * (x8 & 15);
+  for (int x2 = threadIdx.x; x2 < a.group * 64; x2 += kThreads) {  // two dims a thread
+    const int h = x2 >> 6, o2 = 2 * (x2 & 63);
     float M = -INFINITY;
 #pragma unroll
     for (int v = 0; v < kWaves; ++v) M = fmaxf(M, s_ml[(v * a.group + h) * 2]);
-    float L = 0.0f, o[8] = {};
+    float L = 0.0f, o[2] = {};
 #pragma unroll
     for (int v = 0; v < kWaves; ++v) {
       const float m = s_ml[(v * a.group + h) * 2];
       // A wavefront without a visible score has no sums, except where every score was NaN: then its sum is.
       const float e = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - M);
       L += e * s_ml[(v * a.group + h) * 2 + 1];
-      const float* src = s_raw + (v * a.group + h) * kHeadDim + o8;
-#pragma unroll
-      for (int d = 0; d < 8; ++d) o[d] += e * src[d];
+      const float2 src = *reinterpret_cast<const float2*>(s_raw + (v * a.group + h) * kHeadDim + o2);
+      o[0] += e * src.x;
+      o[1] += e * src.y;
     }
     if (whole) {
-      store_bf16x8(out + h * kHeadDim + o8, o, 1.0f / L);
+      *reinterpret_cast<uint32_t*>(out + h * kHeadDim + o2) = pack_bf16x2(o[0] * (1.0f / L), o[1] * (1.0f / L));
     } else {
       const int64_t at = ((b * a.kv_heads + g) * a.group + h) * a.parts + part;
-      float4* dst = reinterpret_cast<float4*>(a.ws_acc + at * kHeadDim + o8);
-      dst[0] = make_float4(o[0], o[1], o[2], o[3]);
-      dst[1] = make_float4(o[4], o[5], o[6], o[7]);
-      if (o8 == 0) *reinterpret_cast<float2*>(a.ws_ml + 2 * at) = make_float2(M, L);
+      *reinterpret_cast<float2*>(a.ws_acc + at * kHeadDim + o2) = make_float2(o[0], o[1]);
+      if (o2 == 0) *reinterpret_cast<float2*>(a.ws_ml + 2 * at) = make_float2(M, L);
     }
   }
 }
