@@ -24,7 +24,8 @@
 // on this card): a wavefront's tile is 1088 cycles of matrix unit and about 270 issue slots of 4 cycles of vector work (32
 // exponentials take four slots each), and the two wavefronts of a SIMD do them largely one after the other.  Timing copies
 // of an earlier 635 us: without the softmax 563, without staging 535, without the products with K 517, with V 485.  No gains:
-// a tile's products a round before its softmax (704 to 708 against 683, instructions interleaved by hand or not),
+// a tile's products a round before its softmax (704 to 708 against 683, instructions interleaved by hand or not; in the narrow
+// form with a third buffer, 2 chunks to 333 behind 1500, 33.7 against 30.0), other XOR patterns of the rows (607 to 617),
 // LDS reads further ahead by hand (709 to 714 against 622), wave priorities (651 against 635), a barrier every two or
 // three tiles (606, 639 against 601), two workgroups of half the queries a CU (630).
 #include <algorithm>
