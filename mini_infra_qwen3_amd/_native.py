@@ -193,6 +193,29 @@ def load() -> ctypes.CDLL:
         return lib
 
 
+_tensor_lists = None
+
+
+def addresses(tensors, like, strided: bool = False) -> ctypes.Array | None:
+    """The addresses of a list or tuple of GPU tensors that all have ``like``'s shape, type and device and are contiguous
+    (``strided``: have its strides), as a C array; None for anything else, which the caller's checks then name."""
+    global _tensor_lists
+    if _tensor_lists is None:
+        import importlib.util
+
+        import torch  # noqa: F401  (its libraries, which the module links)
+
+        path = LIBRARY_PATH.with_name("_tensor_lists.so")
+        if not path.exists():
+            raise NativeLibraryError(f"{path} not found: build it with `python -m mini_infra_qwen3_amd.build`")
+        spec = importlib.util.spec_from_file_location("_tensor_lists", path)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        _tensor_lists = module
+    packed = _tensor_lists.addresses(tensors, like, strided)
+    return None if packed is None else (ctypes.c_void_p * len(tensors)).from_buffer_copy(packed)
+
+
 def check(rc: int, what: str) -> None:
     """Raises the Python error matching a negative ABI status (ValueError for bad arguments)."""
     if rc == MI_OK:

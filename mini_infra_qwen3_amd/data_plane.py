@@ -937,7 +937,15 @@ def copy_blocks(key_pools: Sequence[torch.Tensor], value_pools: Sequence[torch.T
     a pair with a destination outside it is skipped; with ``set_index_checks`` on either raises
     ``IndexError``, and destinations that break the rule above raise ``ValueError``.
     """
-    pool0, device, block_bytes = _record_pools(key_pools, value_pools)
+    keys = values = None
+    if len(key_pools) == len(value_pools) > 0:
+        pool0 = key_pools[0]
+        keys, values = _native.addresses(key_pools, pool0), _native.addresses(value_pools, pool0)
+    if keys is None or values is None or pool0.dim() != 4 or pool0.shape[0] == 0:  # the slow way, which names what is wrong
+        pool0, device, block_bytes = _record_pools(key_pools, value_pools)
+        keys, values = (_native.pointer_array([t.data_ptr() for t in pools]) for pools in (key_pools, value_pools))
+    else:
+        device, block_bytes = pool0.device, pool0.stride(0) * pool0.element_size()
     for name, t in (("src_blocks", src_blocks), ("dst_blocks", dst_blocks)):
         _require_gpu(name, t, device)
         _require_index(name, t, 1)
@@ -954,8 +962,7 @@ def copy_blocks(key_pools: Sequence[torch.Tensor], value_pools: Sequence[torch.T
         if bool(torch.isin(moved, src_blocks).any()):
             raise ValueError("dst_blocks: a block that is written is also a source")
     src_blocks, dst_blocks = src_blocks.contiguous(), dst_blocks.contiguous()
-    _call(device, "mi_copy_blocks", _native.pointer_array([t.data_ptr() for t in key_pools]),
-          _native.pointer_array([t.data_ptr() for t in value_pools]), pool0.shape[0], src_blocks.data_ptr(),
+    _call(device, "mi_copy_blocks", keys, values, pool0.shape[0], src_blocks.data_ptr(),
           dst_blocks.data_ptr(), src_blocks.shape[0], len(key_pools), block_bytes, _stream(device))
 
 
@@ -993,6 +1000,17 @@ def _on_device(device: torch.device, name: str, *args) -> int:
 
 def _call(device: torch.device, name: str, *args) -> None:
     _native.check(_on_device(device, name, *args), name)
+
+
+def _fp4_pool_lists(key_pools: Sequence[torch.Tensor], value_pools: Sequence[torch.Tensor]):
+    """``_require_fp4_pools`` of per-layer lists: the first pool and the addresses of both lists."""
+    pool0 = key_pools[0]
+    keys, values = _native.addresses(key_pools, pool0), _native.addresses(value_pools, pool0)
+    if keys is None or values is None or pool0.dtype is not torch.uint8 or pool0.dim() != 4 or 0 in pool0.shape[1:3] \
+            or pool0.shape[3] != FP4_RECORD_BYTES:
+        _require_fp4_pools(key_pools, value_pools)
+        keys, values = (_native.pointer_array([t.data_ptr() for t in pools]) for pools in (key_pools, value_pools))
+    return pool0, keys, values
 
 
 def _require_fp4_pools(key_pools: Sequence[torch.Tensor], value_pools: Sequence[torch.Tensor]) -> torch.Tensor:
@@ -1038,10 +1056,12 @@ def reshape_and_cache_fp4(
         raise ValueError("reshape_and_cache_fp4: per-layer lists differ in length")
     if num_layers == 0:
         return
-    pool0 = _require_fp4_pools(key_pools, value_pools)
+    pool0, pool_keys, pool_values = _fp4_pool_lists(key_pools, value_pools)
     device, index = pool0.device, pool0.get_device()
     num_blocks, sub, num_kv_heads, _ = pool0.shape
     k0, v0 = key_src[0], value_src[0]
+    src_keys, src_values = _native.addresses(key_src, k0, True), _native.addresses(value_src, v0, True)
+    uniform = src_keys is not None and src_values is not None and k0.get_device() == index == v0.get_device()
     dtype = k0.dtype
     if dtype not in _FP4_SOURCE_TYPES:
         raise ValueError(f"key_src must be bf16, fp16 or fp32, got {dtype}")
@@ -1049,6 +1069,8 @@ def reshape_and_cache_fp4(
         shape, stride = ref.shape, ref.stride()
         if len(shape) != 4 or shape[1] != num_kv_heads or shape[3] != 128:
             raise ValueError(f"{name} must be [B, {num_kv_heads}, L, 128], got {tuple(shape)}")
+        if uniform and ref.dtype is dtype and stride[3] == 1:
+            continue
         for t in tensors:
             if t.get_device() != index:
                 _require_gpu(name, t, device)
@@ -1056,6 +1078,8 @@ def reshape_and_cache_fp4(
                 raise ValueError(f"{name}: all layers need {dtype} and the same shape and strides, with D contiguous")
     if k0.shape != v0.shape:
         raise ValueError("reshape_and_cache_fp4: key and value sources differ in shape")
+    if not uniform:
+        src_keys, src_values = (_native.pointer_array([t.data_ptr() for t in tensors]) for tensors in (key_src, value_src))
     num_tokens = slot_mapping.shape[0] if slot_mapping.ndim else 0
     indices = [slot_mapping, token_rows, token_positions]
     for name, t in zip(("slot_mapping", "token_rows", "token_positions"), indices):
@@ -1076,13 +1100,10 @@ def reshape_and_cache_fp4(
         indices = [None if t is None else t.contiguous() for t in indices]
         index_stride = 1
     slots, rows, positions = indices
-    _call(device, "mi_reshape_and_cache_fp4",
-          _native.pointer_array([t.data_ptr() for t in key_src]), _native.pointer_array([t.data_ptr() for t in value_src]),
+    _call(device, "mi_reshape_and_cache_fp4", src_keys, src_values,
           k0.stride(0), k0.stride(1), k0.stride(2), v0.stride(0), v0.stride(1), v0.stride(2),
           rows.data_ptr() if rows is not None else None, positions.data_ptr() if positions is not None else None,
-          slots.data_ptr(), index_stride, num_tokens, k0.shape[0], k0.shape[2],
-          _native.pointer_array([t.data_ptr() for t in key_pools]),
-          _native.pointer_array([t.data_ptr() for t in value_pools]), num_layers,
+          slots.data_ptr(), index_stride, num_tokens, k0.shape[0], k0.shape[2], pool_keys, pool_values, num_layers,
           num_blocks * sub * KERNEL_BLOCK_SIZE, num_kv_heads, 128, _FP4_SOURCE_TYPES[dtype], _stream(device))
 
 
@@ -1103,19 +1124,25 @@ def gather_blocks_fp4(
         raise ValueError("gather_blocks_fp4: per-layer lists differ in length")
     if num_layers == 0:
         return
-    pool0 = _require_fp4_pools(key_pools, value_pools)
+    pool0, pool_keys, pool_values = _fp4_pool_lists(key_pools, value_pools)
     device, index = pool0.device, pool0.get_device()
     _require_gpu("block_ids", block_ids, device)
     _require_index("block_ids", block_ids, 2)
     num_blocks, sub, num_kv_heads, _ = pool0.shape
     batch, nb = block_ids.shape
     expect = (batch, nb * sub * KERNEL_BLOCK_SIZE, num_kv_heads, 128)
-    for name, tensors in (("key_out", key_out), ("value_out", value_out)):
+    out0 = key_out[0]
+    out_keys, out_values = _native.addresses(key_out, out0), _native.addresses(value_out, out0)
+    uniform = out_keys is not None and out_values is not None and out0.shape == expect and out0.dtype is torch.bfloat16 \
+        and out0.get_device() == index
+    for name, tensors in () if uniform else (("key_out", key_out), ("value_out", value_out)):
         for t in tensors:
             if t.get_device() != index:
                 _require_gpu(name, t, device)
             if t.shape != expect or t.dtype is not torch.bfloat16 or not t.is_contiguous():
                 raise ValueError(f"{name}: expected contiguous {expect} bf16, got {tuple(t.shape)} {t.dtype}")
+    if not uniform:
+        out_keys, out_values = (_native.pointer_array([t.data_ptr() for t in tensors]) for tensors in (key_out, value_out))
     if batch == 0 or nb == 0:
         return
     _check_range("block_ids", block_ids, num_blocks)
@@ -1123,11 +1150,9 @@ def gather_blocks_fp4(
         block_ids, num_blocks, nb = _fp4_sub_block_ids(block_ids, num_blocks, sub), num_blocks * sub, nb * sub
     if block_ids.stride(1) != 1 or (batch > 1 and block_ids.stride(0) < nb):
         block_ids = block_ids.contiguous()
-    _call(device, "mi_gather_blocks_fp4", _native.pointer_array([t.data_ptr() for t in key_pools]),
-          _native.pointer_array([t.data_ptr() for t in value_pools]), num_blocks, block_ids.data_ptr(),
+    _call(device, "mi_gather_blocks_fp4", pool_keys, pool_values, num_blocks, block_ids.data_ptr(),
           block_ids.stride(0) if batch > 1 else nb, batch, nb,
-          _native.pointer_array([t.data_ptr() for t in key_out]), _native.pointer_array([t.data_ptr() for t in value_out]),
-          num_layers, num_kv_heads, 128, _stream(device))
+          out_keys, out_values, num_layers, num_kv_heads, 128, _stream(device))
 
 
 def _workspace(workspace: torch.Tensor | None, need: int, device: torch.device) -> tuple[int | None, int, torch.Tensor | None]:
