@@ -1,7 +1,7 @@
 // Checks of per-layer tensor lists in one call: the data plane's entry points take a key and a value pool (and sources or
 // outputs) of every layer, and asking Python for shape, type, layout, device and address of each took most of a small
-// call's time (56 pools of 28 layers: a block copy whose kernel takes 5 us
-// took 21, and takes 7 with this; a gather of 112 tensors and 11 us took 35, and takes 10 to 11).
+// call's time.  56 pools of 28 layers: a block copy whose kernel takes 5 us took 21, and takes 7 with this; a gather over
+// 112 tensors whose kernel takes 11 took 35, and takes 10 to 11.
 //
 // A CPython module beside the C ABI library, which knows no torch type.  It decides nothing: a list that is not uniform
 // comes back as None, and the caller's own checks say what is wrong with it.
