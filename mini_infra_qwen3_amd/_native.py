@@ -196,9 +196,7 @@ def load() -> ctypes.CDLL:
 _tensor_lists = None
 
 
-def addresses(tensors, like, strided: bool = False) -> ctypes.Array | None:
-    """The addresses of a list or tuple of GPU tensors that all have ``like``'s shape, type and device and are contiguous
-    (``strided``: have its strides), as a C array; None for anything else, which the caller's checks then name."""
+def _packed_addresses(tensors, like, strided: bool) -> bytes | None:
     global _tensor_lists
     if _tensor_lists is None:
         import importlib.util
@@ -212,7 +210,18 @@ def addresses(tensors, like, strided: bool = False) -> ctypes.Array | None:
         module = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(module)
         _tensor_lists = module
-    packed = _tensor_lists.addresses(tensors, like, strided)
+    return _tensor_lists.addresses(tensors, like, strided)
+
+
+def uniform(tensors, like) -> bool:
+    """Whether a list or tuple holds contiguous GPU tensors of ``like``'s shape, type and device alone."""
+    return _packed_addresses(tensors, like, False) is not None
+
+
+def addresses(tensors, like, strided: bool = False) -> ctypes.Array | None:
+    """The addresses of a list or tuple of GPU tensors that all have ``like``'s shape, type and device and are contiguous
+    (``strided``: have its strides), as a C array; None for anything else, which the caller's checks then name."""
+    packed = _packed_addresses(tensors, like, strided)
     return None if packed is None else (ctypes.c_void_p * len(tensors)).from_buffer_copy(packed)
 
 

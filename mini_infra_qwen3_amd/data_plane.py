@@ -1013,6 +1013,14 @@ def _fp4_pool_lists(key_pools: Sequence[torch.Tensor], value_pools: Sequence[tor
     return pool0, keys, values
 
 
+def _require_fp4_pool(key_pool: torch.Tensor, value_pool: torch.Tensor) -> None:
+    """``_require_fp4_pools`` of one layer."""
+    shape = key_pool.shape
+    if not _native.uniform((key_pool, value_pool), key_pool) or key_pool.dtype is not torch.uint8 or len(shape) != 4 \
+            or shape[3] != FP4_RECORD_BYTES or shape[1] < 1 or shape[2] < 1:
+        _require_fp4_pools((key_pool,), (value_pool,))
+
+
 def _require_fp4_pools(key_pools: Sequence[torch.Tensor], value_pools: Sequence[torch.Tensor]) -> torch.Tensor:
     """Checks 4-bit pools (one shape, one device, contiguous uint8); returns the first."""
     pool0 = key_pools[0]
@@ -1192,8 +1200,8 @@ def paged_decode_attention_fp4(
     ``[B, H * 128]`` bf16.  ``workspace`` (optional, uint8, reused across calls of one stream) holds the partials of
     long contexts; it is allocated here when missing or too small.
     """
-    pool0 = _require_fp4_pools((key_pool,), (value_pool,))
-    device, index = pool0.device, pool0.get_device()
+    _require_fp4_pool(key_pool, value_pool)
+    device, index = key_pool.device, key_pool.get_device()
     for name, t in (("query", query), ("block_tables", block_tables), ("context_lens", context_lens)):
         if t.get_device() != index:
             _require_gpu(name, t, device)
@@ -1202,7 +1210,7 @@ def paged_decode_attention_fp4(
     if query.ndim != 3 or query.dtype is not torch.bfloat16 or query.stride(2) != 1 or query.shape[2] != 128:
         raise ValueError(f"query must be [B, H, 128] bf16 with D contiguous, got {tuple(query.shape)} {query.dtype}")
     batch, num_heads, head_dim = query.shape
-    num_blocks, sub, num_kv_heads, _ = pool0.shape
+    num_blocks, sub, num_kv_heads, _ = key_pool.shape
     if block_tables.shape[0] != batch or context_lens.shape[0] != batch:
         raise ValueError("block_tables / context_lens batch differs from query batch")
     if out is None:
@@ -1267,8 +1275,8 @@ def chunked_prefill_attention_fp4(
     row b is the ``chunk_lens[b]`` tokens from ``chunk_first[b]`` on, at most ``max_len``; rows do not overlap.  ``out``
     ``[1, C, H * 128]`` then keeps what it held where no row is (zeros, if it is allocated here).
     """
-    pool0 = _require_fp4_pools((key_pool,), (value_pool,))
-    device, index = pool0.device, pool0.get_device()
+    _require_fp4_pool(key_pool, value_pool)
+    device, index = key_pool.device, key_pool.get_device()
     ragged = chunk_first is not None
     if ragged:
         if max_len is None or max_len < 0:
@@ -1286,7 +1294,7 @@ def chunked_prefill_attention_fp4(
         if t.ndim != 4 or t.dtype is not torch.bfloat16 or t.stride(3) != 1 or t.shape[3] != 128:
             raise ValueError(f"{name} must be 4-d bf16 with a contiguous last dim of 128, got {tuple(t.shape)} {t.dtype}")
     batch, num_heads, padded_len, head_dim = query.shape
-    num_blocks, sub, num_kv_heads, _ = pool0.shape
+    num_blocks, sub, num_kv_heads, _ = key_pool.shape
     if key.shape != (batch, num_kv_heads, padded_len, head_dim) or value.shape != key.shape:
         raise ValueError(f"key/value must be [{batch}, {num_kv_heads}, {padded_len}, {head_dim}]")
     tensor_rows = batch
